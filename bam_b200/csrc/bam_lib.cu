@@ -971,7 +971,7 @@ static int cache_reset_device(bam_cache* pc)
 static void cache_free_device(bam_cache* pc)
 {
     page_cache_d_t& d = pc->d;
-    cudaFree(d.base_addr); cudaFree(d.slots); cudaFree(d.table); cudaFree(d.clock_hand);
+    cudaFree(pc->base_raw); cudaFree(d.slots); cudaFree(d.table); cudaFree(d.clock_hand);
     cudaFree(d.stats); cudaFree(d.range_page_starts); cudaFree(d.range_dists); cudaFree(pc->prp_lists_raw);
     cudaFree(d.d_ctrls); cudaFree(pc->d_group_qps);
 }
@@ -1030,7 +1030,10 @@ extern "C" int bam_cache_create_multi(bam_cache_t* out, const bam_ctrl_t* ctrls,
     for (uint32_t k = 0; k < n_ctrls; k++) total_qps += ctrls[k]->n_qps;
     cudaError_t e = cudaSuccess;
     auto alloc = [&](void** p, size_t bytes) { if (e == cudaSuccess) e = cudaMalloc(p, bytes); };
-    alloc((void**)&d.base_addr, n_pages * (size_t)page_size);
+    /* Slots lie on controller pages: a PRP that starts inside one is continued at PRP2, and pages of up to 4096 bytes
+     * are submitted without a PRP2.  cudaMalloc itself promises 256 bytes. */
+    alloc(&pc->base_raw, n_pages * (size_t)page_size + 4096);
+    d.base_addr = reinterpret_cast<uint8_t*>(((uintptr_t)pc->base_raw + 4095) / 4096 * 4096);
     alloc((void**)&d.slots, n_pages * sizeof(bam_slot_t));
     alloc((void**)&d.table, pc->n_buckets * BAM_BUCKET_WORDS * 4);
     alloc((void**)&d.clock_hand, 8 * BAM_HAND_STRIDE * BAM_MAX_HANDS);
