@@ -8,3 +8,4 @@ from .host import (REPLICATE, STRIPE, Array, Controller, PageCache, backing_loca
                    direct_checksum, gen_block_pages, page_sums, place_rank, probe_uplink_groups, shard_pages, spread_over_uplinks, zipf_cdf)
 from .graph import (CsrGraph, DistCsrGraph, build_rmat_csr, load_bel_graph, read_bel, write_bel, allreduce_min_u32, u32_less, gather_headers, raise_on_rank_failure,  # noqa: F401,E402
                     rmat_thresholds, shard_vertices, shard_vertices_by_edges)
+from .kv import KvCache  # noqa: F401,E402

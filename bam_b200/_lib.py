@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 # BAM_B200_LIB selects another build of the same library (e.g. one compiled with -DBAM_PROFILE)
 LIB_PATH = os.environ.get("BAM_B200_LIB") or os.path.join(HERE, "libbam_b200.so")
 
-u32, u64, vp, ci = C.c_uint32, C.c_uint64, C.c_void_p, C.c_int
+u32, u64, i64, vp, ci = C.c_uint32, C.c_uint64, C.c_int64, C.c_void_p, C.c_int
 
 
 class CacheStats(C.Structure):
@@ -23,6 +23,24 @@ class RangeDesc(C.Structure):
 
 class StatusOut(C.Structure):
     _fields_ = [("code", u32), ("where", u32), ("detail", u64)]
+
+
+class KvLayout(C.Structure):
+    _fields_ = [("dtype", u32), ("head_dim", u32), ("n_kv_heads", u32), ("block_tokens", u32), ("n_blocks", u64),
+                ("first_page", u64)]
+
+
+class KvAppend(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("q_out", vp), ("q_stride", i64 * 2), ("k_stride", i64 * 2),
+                ("v_stride", i64 * 2), ("q_out_stride", i64 * 2), ("n_tokens", u64), ("slots", vp), ("positions", vp),
+                ("cos", vp), ("sin", vp), ("n_positions", u64), ("rope_stride", i64), ("q_norm", vp), ("k_norm", vp),
+                ("n_q_heads", u32), ("rotary_dim", u32), ("rope_style", u32), ("norm_eps", C.c_float)]
+
+
+class KvAttend(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("lse", vp), ("q_stride", i64 * 2), ("out_stride", i64 * 2), ("block_table", vp),
+                ("seq_lens", vp), ("table_stride", i64), ("window", i64), ("sinks", i64), ("batch", u32), ("n_q_heads", u32),
+                ("table_width", u32), ("scale", C.c_float)]
 
 
 # name -> (restype, argtypes); mirrors include/bam_abi.h one to one
@@ -87,6 +105,10 @@ SIGNATURES = {
     "bam_launch_pr_sweep": (ci, [vp, vp, u64, u64, u64, vp, vp, vp, vp, vp, u64, vp]),
     "bam_launch_degrees": (ci, [vp, u64, vp, vp]),
     "bam_pagerank_run": (ci, [vp, vp, u64, u64, u64, u64, u32, vp, C.POINTER(u32), C.POINTER(u64)]),
+    "bam_kv_scratch_bytes": (u64, [vp, C.POINTER(KvLayout)]),
+    "bam_launch_kv_append": (ci, [vp, C.POINTER(KvLayout), C.POINTER(KvAppend), vp, u64, vp]),
+    "bam_launch_kv_gather": (ci, [vp, C.POINTER(KvLayout), u64, vp, vp, vp, C.POINTER(i64), C.POINTER(i64), vp, u64, vp]),
+    "bam_launch_kv_attend": (ci, [vp, C.POINTER(KvLayout), C.POINTER(KvAttend), vp, u64, vp]),
     "bam_gen_rmat_keys": (ci, [vp, u64, u64, u64, u32, u32, u32, u32, vp]),
     "bam_ctrl_write_store_from_device": (ci, [vp, u64, vp, u64, vp]),
     "bam_gen_uniform_indices": (ci, [vp, u64, u64, u64, u64, vp]),

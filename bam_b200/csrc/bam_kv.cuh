@@ -1,0 +1,109 @@
+/*
+ * bam_kv.cuh -- rows of a key/value cache inside the pages of an array.
+ *
+ * A page of the array holds the keys and then the values of one block of `block_tokens` consecutive tokens for
+ * ONE key/value head: page = first_page + block * n_kv_heads + head, and inside it
+ *
+ *     K[block_tokens][head_dim]  V[block_tokens][head_dim]          (16-bit elements)
+ *
+ * so that what one head needs of a block is one contiguous piece: one look-up, one pin, two bulk copies.
+ * The 16-byte chunks of a row are permuted by the row's number (swizzle, below): eight consecutive rows then put
+ * the same logical chunk on eight different 16-byte bank groups of shared memory, and the matrix loads of the
+ * attention kernel read a page's verbatim copy without bank conflicts -- nobody has to permute on the way in.
+ */
+#ifndef BAM_KV_CUH
+#define BAM_KV_CUH
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "bam_abi.h"
+#include "bam_fused.cuh"
+
+namespace bam {
+
+/* A launch's own words at the head of its scratch, all ones when the launch starts (one memset, so a captured
+ * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks.
+ * An index outside its range is noted in `bad` and goes into the status block by the last worker block: a status
+ * that is set earlier makes every wait of the launch give up, and a page whose fetch is given up is lost to the cache. */
+struct kv_launch_words_t {
+    uint32_t remaining, done, bad, pad0;
+    uint64_t bad_index;
+    uint32_t pad[10];
+};
+
+/* what a kernel knows of the layout */
+struct kv_layout_d_t {
+    range_d_t<uint64_t> r;
+    uint64_t first_page, n_blocks;
+    uint32_t head_dim, n_kv_heads, block_tokens;
+    uint32_t chunks;                 /* 16-byte chunks of a row: head_dim / 8                 */
+    uint32_t swz_shift, swz_mask;    /* see swizzle                                           */
+    kv_launch_words_t* words;
+
+    BAM_DEV void bad_index(uint64_t i) const { if (atom_cas_relaxed(&words->bad, 0xffffffffu, 1u) == 0xffffffffu) words->bad_index = i; }
+    BAM_DEV uint64_t page_of(uint64_t block, uint32_t head) const { return first_page + block * n_kv_heads + head; }
+    BAM_DEV uint32_t row_bytes() const { return head_dim * 2u; }
+    BAM_DEV uint32_t v_offset() const { return block_tokens * head_dim * 2u; }
+    /* Rows lie head_dim / 8 chunks apart.  With a multiple of 8 every row starts on the same bank group, so the
+     * chunk number is XORed with the row's low three bits; with 4 mod 8 two rows make one round of the bank groups
+     * and bits 2:1 of the row suffice, with 2 mod 4 bit 2.  An odd number needs none.  The mask's range divides
+     * the number of chunks, so the result is a chunk of the same row. */
+    BAM_DEV uint32_t swizzle(uint32_t row, uint32_t chunk) const { return chunk ^ ((row >> swz_shift) & swz_mask); }
+};
+
+template <class T> struct kv_type;
+template <> struct kv_type<__nv_bfloat16> {
+    static BAM_DEV float to_f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+    static BAM_DEV uint32_t pack(float lo, float hi) { __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&p); }
+    static BAM_DEV float2 unpack(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+};
+template <> struct kv_type<__half> {
+    static BAM_DEV float to_f(uint16_t b) { return __half2float(__ushort_as_half(b)); }
+    static BAM_DEV uint32_t pack(float lo, float hi) { __half2 p = __floats2half2_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&p); }
+    static BAM_DEV float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+};
+
+/* Eight elements from memory of any 2-byte alignment; `vec`: 16-byte aligned. */
+BAM_DEV uint4 kv_load8(const uint16_t* p, bool vec)
+{
+    if (vec) return *reinterpret_cast<const uint4*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+BAM_DEV void kv_store8(uint16_t* p, uint4 v, bool vec)
+{
+    if (vec) { *reinterpret_cast<uint4*>(p) = v; return; }
+    const uint32_t w[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+    for (int i = 0; i < 4; i++) { p[2 * i] = (uint16_t)w[i]; p[2 * i + 1] = (uint16_t)(w[i] >> 16); }
+}
+
+/* The fused launch of these operators.  Like bam_fused, but the words that end the controller blocks belong to
+ * the launch and not to the controller, so that launches on one controller may overlap and a captured launch can
+ * be replayed: worker blocks count up from all-ones, and the last one clears `remaining`. */
+template <class Work>
+__global__ void __launch_bounds__(Work::threads, Work::min_blocks)
+bam_kv_fused(const __grid_constant__ bam_emu_d_t emu, const __grid_constant__ Work work)
+{
+    if (blockIdx.x < emu.n_ctrl_blocks) {
+        emu_controller_main(emu, bam_dyn_smem);
+        return;
+    }
+    const uint32_t n_work = gridDim.x - emu.n_ctrl_blocks;
+    work(blockIdx.x - emu.n_ctrl_blocks, n_work);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        kv_launch_words_t* w = reinterpret_cast<kv_launch_words_t*>(emu.consumers_remaining);
+        __threadfence();
+        if (atom_add_acq_rel(&w->done, 1u) == n_work - 2u) {
+            if (ld_relaxed_gpu(&w->bad) == 1u) status_fail(emu.status, BAM_ERANGE, BAM_AT_RANGE, ld_relaxed_gpu(&w->bad_index));
+            st_release_scoped(&w->remaining, 0u, emu.sys_scope != 0);
+        }
+    }
+}
+
+}  // namespace bam
+#endif

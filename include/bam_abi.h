@@ -352,6 +352,77 @@ int bam_gen_rmat_keys(uint64_t* keys_dev, uint64_t e_begin, uint64_t e_end, uint
  * benchmarks/readwrite/main.cu:283-316). */
 int bam_ctrl_write_store_from_device(bam_ctrl_t c, uint64_t byte_offset, const void* src_dev, uint64_t bytes, void* stream);
 
+/* ---- key/value cache in the pages of an array ----------------------------------------------------------
+ * No counterpart in the reference.  The keys and values of attention heads, kept in the pages of an array of one
+ * range: a page holds the block of `block_tokens` consecutive tokens of ONE key/value head, first the keys, then the
+ * values, page = first_page + block * n_kv_heads + head.  A token's slot is block * block_tokens + its place in the
+ * block.  Within a row of head_dim 16-bit elements the 16-byte chunk c of row r lies at chunk c ^ ((r >> a) & b):
+ * a = 0, b = 7 if head_dim / 8 is a multiple of 8; a = 1, b = 3 if of 4; a = 2, b = 1 otherwise.  Pages that are not
+ * in the cache are fetched, and dirty ones written back, by the launch that needs them.
+ *
+ * head_dim: a multiple of 16, at most 256; block_tokens: a multiple of 16 with block_tokens * head_dim * 4 <= the page.
+ * Strides are in elements: [0] from token (or sequence) to token, [1] from head to head; a head's elements are
+ * contiguous.  Every launch is asynchronous on `stream`, may be captured into a CUDA graph, and leaves the calling
+ * thread's device as it was.  scratch_dev: bam_kv_scratch_bytes bytes of device memory, 128-byte aligned, that nothing
+ * else uses until the launch has finished (a captured launch keeps using it: every graph needs its own); its contents
+ * need no initialisation.  An index outside its range (a slot, position, block or length) is not followed: the status
+ * block says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has finished, the rows that it concerns are undefined. */
+#define BAM_KV_BF16 0u
+#define BAM_KV_FP16 1u
+#define BAM_KV_ROPE_HALF 0u      /* pairs (i, i + rotary_dim / 2) */
+#define BAM_KV_ROPE_PAIRS 1u     /* pairs (2 i, 2 i + 1)          */
+typedef struct {
+    uint32_t dtype, head_dim, n_kv_heads, block_tokens;
+    uint64_t n_blocks;
+    uint64_t first_page;         /* page of the array that block 0, head 0 is (a layer's share of the array starts there) */
+} bam_kv_layout_t;
+uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* layout);
+
+/* Append: row t of k and v goes to slots[t] (int64; negative: the row is padding and nothing is written; a slot that
+ * appears twice keeps either row).  On the way each head of k, and of q where it is given, is
+ *   normed:   y = x * rsqrt(mean(x^2) + norm_eps) * w      (q_norm / k_norm: head_dim elements of the layout's type, or NULL)
+ *   rotated:  (a, b) -> (a c - b s, b c + a s) over the first rotary_dim (a multiple of 16) elements, with c and s the
+ *             floats cos / sin[positions[t] * rope_stride + i] of pair i (cos NULL: no rotation; positions int64, below
+ *             n_positions; that of a padding row is clamped)
+ * in 32 bits and rounded once; v is copied.  q_out may be q. */
+typedef struct {
+    const void *q, *k, *v;
+    void* q_out;
+    int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2];
+    uint64_t n_tokens;
+    const int64_t *slots, *positions;
+    const float *cos, *sin;
+    uint64_t n_positions;
+    int64_t rope_stride;
+    const void *q_norm, *k_norm;
+    uint32_t n_q_heads, rotary_dim, rope_style;
+    float norm_eps;
+} bam_kv_append_t;
+int bam_launch_kv_append(bam_array_t a, const bam_kv_layout_t* layout, const bam_kv_append_t* args, void* scratch_dev,
+                         uint64_t scratch_bytes, void* stream);
+/* Gather: k_out and v_out row t = the row at slots[t] (zeros for a negative slot). */
+int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t n_tokens, const int64_t* slots_dev,
+                         void* k_out_dev, void* v_out_dev, const int64_t* k_stride, const int64_t* v_stride,
+                         void* scratch_dev, uint64_t scratch_bytes, void* stream);
+/* Attention of one new token per sequence over its cached tokens:
+ *   out[b, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[b, h] . k_j - max),  lse[b, h] = max + log(sum_j p_j)
+ * over the tokens j < seq_lens[b] (int32) that are visible: all of them, or with window > 0 the last `window` and the
+ * first `sinks`.  Query head h reads key/value head h / (n_q_heads / n_kv_heads).  Token j of sequence b lies in block
+ * block_table[b * table_stride + j / block_tokens] (int32); entries of blocks without a visible token are not read.
+ * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL). */
+typedef struct {
+    const void* q;
+    void* out;
+    float* lse;
+    int64_t q_stride[2], out_stride[2];
+    const int32_t *block_table, *seq_lens;
+    int64_t table_stride, window, sinks;
+    uint32_t batch, n_q_heads, table_width;
+    float scale;
+} bam_kv_attend_t;
+int bam_launch_kv_attend(bam_array_t a, const bam_kv_layout_t* layout, const bam_kv_attend_t* args, void* scratch_dev,
+                         uint64_t scratch_bytes, void* stream);
+
 /* ---- synthetic access streams ------------------------------------------------------------------
  * The reference benchmarks build their access lists on the host with rand()
  * (benchmarks/array/main.cu:150-162, benchmarks/pattern/main.cu:560-600); these write the seeded
