@@ -50,6 +50,7 @@
 #define BAM_AT_RANGE 11       /* index outside every range of the array     */
 #define BAM_AT_TMA 12         /* bulk-copy mbarrier wait                    */
 #define BAM_AT_LAUNCH 13      /* the whole launch outlived launch_timeout_ns */
+#define BAM_AT_KV_JOIN 15     /* attention: a block waited for another's part of a split sequence */
 #define BAM_AT_SQ_ORDER 14    /* controller: an earlier batch of the queue never handed its entries back */
 
 /* Per-controller error/status block in device memory.  code is written once (first error
