@@ -2,12 +2,15 @@
 import os
 import shutil
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbam_b200.so")
-SOURCES = ["bam_lib.cu", "bam_noalloc.cu", "bam_graph.cu", "bam_exchange.cu", "bam_nvm_host.cu", "bam_kv.cu"]
+SOURCES = ["bam_lib.cu", "bam_noalloc.cu", "bam_graph.cu", "bam_exchange.cu", "bam_nvm_host.cu", "bam_kv.cu", "bam_kv_attend_bf16.cu",
+           "bam_kv_attend_fp16.cu"]
 
 
 def _newer_than(target, deps):
@@ -39,18 +42,23 @@ def build_library(force=False, verbose=False, profile=False):
     lib = PROFILE_LIB if profile else LIB
     if not force and not _newer_than(lib, _deps()):
         return lib
-    cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-Xptxas", "-v", "-shared", "-Xcompiler", "-fPIC"] + (["-DBAM_PROFILE"] if profile else []) + [
-           "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-o", lib + ".tmp"]
-    cmd += [os.path.join(CSRC, s) for s in SOURCES]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode == 0:
-        os.replace(lib + ".tmp", lib)          # a reader never sees a half-written library
-    if verbose or res.returncode != 0:
-        print(res.stdout)
-        print(res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed building " + os.path.basename(lib))
+    flags = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
+    flags += (["-DBAM_PROFILE"] if profile else []) + ["-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
+
+    def run(cmd):
+        res = subprocess.run([nvcc_path()] + cmd, capture_output=True, text=True)
+        if verbose or res.returncode != 0:
+            print(res.stdout)
+            print(res.stderr)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed building " + os.path.basename(lib))
+
+    # the sources do not depend on one another: one nvcc each, side by side, then one link
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(min(len(SOURCES), os.cpu_count() or 1)) as pool:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        list(pool.map(lambda so: run(flags + ["-Xptxas", "-v", "-c", os.path.join(CSRC, so[0]), "-o", so[1]]), zip(SOURCES, objs)))
+        run(["-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", lib + ".tmp"] + objs)
+    os.replace(lib + ".tmp", lib)              # a reader never sees a half-written library
     return lib
 
 

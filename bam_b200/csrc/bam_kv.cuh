@@ -22,6 +22,8 @@
 
 namespace bam {
 
+#define KV_ROWS 16u                   /* query heads of a unit of the attention: the rows of a matrix instruction */
+
 /* A launch's own words at the head of its scratch, all ones when the launch starts (one memset, so a captured
  * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks.
  * An index outside its range is noted in `bad` and goes into the status block by the last worker block: a status
@@ -104,6 +106,74 @@ bam_kv_fused(const __grid_constant__ bam_emu_d_t emu, const __grid_constant__ Wo
         }
     }
 }
+
+/* ---- host side ------------------------------------------------------------------------------------------ */
+
+
+/* The calling thread's device is the caller's affair: it is put back when the entry point returns. */
+struct device_guard {
+    int was = -1;
+    cudaError_t enter(int dev)
+    {
+        cudaError_t e = cudaGetDevice(&was);
+        if (e == cudaSuccess && was != dev) e = cudaSetDevice(dev);
+        return e;
+    }
+    ~device_guard()
+    {
+        int now = -1;
+        if (was >= 0 && cudaGetDevice(&now) == cudaSuccess && now != was) (void)cudaSetDevice(was);
+    }
+};
+
+/* Blocks of a kernel that are co-resident on the current device, and the shared memory attribute: asked once. */
+template <class Work>
+cudaError_t kv_max_grid(int dev, uint32_t* grid)
+{
+    static uint32_t known[64] = {};                  /* the same value whoever writes it */
+    if (dev < 64 && known[dev]) { *grid = known[dev]; return cudaSuccess; }
+    int sms = 0, nb = 0;
+    cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(bam_kv_fused<Work>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Work::smem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&nb, bam_kv_fused<Work>, Work::threads, Work::smem);
+    if (e != cudaSuccess) return e;
+    *grid = (uint32_t)nb * (uint32_t)sms;
+    if (dev < 64) known[dev] = *grid;
+    return cudaSuccess;
+}
+
+/* Launch with at most `want` worker blocks.  The launch's words are the first bytes of `scratch`; `clear` bytes of
+ * it are set to all ones. */
+template <class Work>
+int kv_launch(bam_ctrl* c, const Work& work, uint64_t want, void* scratch, size_t clear, cudaStream_t s)
+{
+    uint32_t grid = 0;
+    CK(kv_max_grid<Work>(c->device, &grid));
+    if (c->max_grid && grid > c->max_grid) grid = c->max_grid;
+    bam_emu_d_t emu = c->emu;
+    if (want == 0) want = 1;
+    /* few workers need few command processors, and a small grid starts and ends sooner */
+    if (emu.n_ctrl_blocks > 4 && emu.n_ctrl_blocks > want) emu.n_ctrl_blocks = want > 4 ? (uint32_t)want : 4u;
+    if (grid <= emu.n_ctrl_blocks) return BAM_EINVAL;
+    if (grid - emu.n_ctrl_blocks > want) grid = emu.n_ctrl_blocks + (uint32_t)want;
+    emu.consumers_remaining = reinterpret_cast<uint32_t*>(scratch);
+    Work w = work;
+    w.L.words = reinterpret_cast<kv_launch_words_t*>(scratch);
+    CK(cudaMemsetAsync(scratch, 0xff, clear, s));
+    void* args[] = { (void*)&emu, (void*)&w };
+    CK(cudaLaunchCooperativeKernel((const void*)bam_kv_fused<Work>, dim3(grid), dim3(Work::threads), args, Work::smem, s));
+    return BAM_OK;
+}
+
+/* Scratch: the launch's words, a counter per worker block, the blocks' parts. */
+inline uint32_t kv_most_blocks(bam_array* a) { return (uint32_t)a->pc->ctrl->num_sms * 2u; }
+inline size_t kv_parts_at(uint32_t blocks) { return (sizeof(kv_launch_words_t) + 4 * (size_t)blocks + 127) / 128 * 128; }
+
+/* The attention's launchers, one translation unit per element type. */
+template <class T>
+int kv_launch_attend(bam_array* a, const kv_layout_d_t& L, const bam_kv_attend_t* p, void* scratch, void* stream);
+extern template int kv_launch_attend<__nv_bfloat16>(bam_array*, const kv_layout_d_t&, const bam_kv_attend_t*, void*, void*);
+extern template int kv_launch_attend<__half>(bam_array*, const kv_layout_d_t&, const bam_kv_attend_t*, void*, void*);
 
 }  // namespace bam
 #endif

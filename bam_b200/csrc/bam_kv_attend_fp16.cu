@@ -1,0 +1,4 @@
+/* bam_kv_attend_fp16.cu -- the attention kernels for __half rows (see bam_kv_attend.cuh) */
+#include "bam_kv_attend.cuh"
+
+template int bam::kv_launch_attend<__half>(bam_array*, const bam::kv_layout_d_t&, const bam_kv_attend_t*, void*, void*);
