@@ -96,18 +96,16 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
     bool pending = want;
     spin_t sp;
     while (__any_sync(full, pending)) {
-        /* rows of one page share a pin (the coalescing of the array reads) */
-        const uint32_t eq = __match_any_sync(full, pending ? page : ~(uint64_t)lane);
-        const uint32_t leader = __ffs(eq) - 1, cnt = __popc(eq);
-        uint32_t slot = L.r.acquire_page_warp(full, pending && lane == leader, pending ? page : 0, cnt, write, queue);
-        slot = __shfl_sync(full, slot, leader);
+        const uint32_t slot = kv_pin_warp(L, pending, page, write, queue);
         const bool got = pending && slot <= BAM_SLOT_MAX;
         const bool failed = __any_sync(full, pending && slot == BAM_SLOT_ERR);
         const uint32_t m = __ballot_sync(full, got);
         if (m && !failed) rows(m, got ? L.r.get_cache_page_addr(slot) : 0);
         if (write) __threadfence();
         __syncwarp();
-        if (got && lane == leader) L.r.release_page(slot, cnt);
+        /* one release per page: the lowest of the lanes that share it gives all their counts back */
+        const uint32_t same = __match_any_sync(full, got ? slot : ~lane);
+        if (got && lane == (uint32_t)(__ffs(same) - 1)) L.r.release_page(slot, __popc(same));
         if (failed) return false;
         if (got) pending = false;
         if (m == 0u && __any_sync(full, sp.expired(L.r.cache.status, BAM_AT_FIND_SLOT, page))) return false;

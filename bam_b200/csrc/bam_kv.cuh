@@ -66,6 +66,26 @@ template <> struct kv_type<__half> {
     static BAM_DEV float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 };
 
+/* Pin a page per lane: every lane calls it, lanes that want the same page share one fetch-add (each releases its own
+ * count of one).  What is resident is pinned at once; the warp asks the cache's miss path for the rest. */
+BAM_DEV uint32_t kv_pin_warp(const kv_layout_d_t& L, bool want, uint64_t page, bool write, uint32_t queue)
+{
+    const uint32_t full = 0xffffffffu, lane = lane_id();
+    const uint32_t eq = __match_any_sync(full, want ? page : ~(uint64_t)lane);
+    const uint32_t leader = __ffs(eq) - 1, cnt = __popc(eq);
+    const bool ask = want && lane == leader;
+    uint32_t slot = BAM_SLOT_ERR;
+    if (ask) slot = cache_try_pin(L.r.cache, L.r.get_global_address(page), cnt, write);
+    const uint32_t hits = __reduce_add_sync(full, ask && slot <= BAM_SLOT_MAX ? cnt : 0u);
+    if (hits && lane == 0) count_hit(L.r.cache, hits);
+    const bool more = ask && slot == BAM_SLOT_NONE;
+    if (__any_sync(full, more)) {
+        const uint32_t x = L.r.acquire_page_warp(full, more, more ? page : 0, cnt, write, queue);
+        if (more) slot = x;
+    }
+    return __shfl_sync(full, slot, leader);
+}
+
 /* Eight elements from memory of any 2-byte alignment; `vec`: 16-byte aligned. */
 BAM_DEV uint4 kv_load8(const uint16_t* p, bool vec)
 {

@@ -209,7 +209,7 @@ struct KvAttendWork {
             base_pos = __shfl_sync(full_mask, pos, 31) + 1;
             const uint32_t k = (uint32_t)(f - f0) + lane, place = k % KV_AHEAD, round = k / KV_AHEAD;
             if (!wait(sh, [&] { return __all_sync(full_mask, !pending || ld_acquire_cta(&sh.tag[place]) == 2u * round); })) return;
-            /* pin: chunks of one page share a fetch-add.  A lane whose page cannot be had now is asked for again when
+            /* A lane whose page cannot be had now is asked for again when
              * the chunks before it have been handed on, and the chunks behind it give theirs back meanwhile: what a
              * block holds is always the next it needs, so blocks never wait for pages that wait for them */
             sp.reset();
@@ -219,10 +219,7 @@ struct KvAttendWork {
                 if (todo == 0u) break;
                 const uint32_t upto = __ffs(todo) - 1 + ask;
                 const bool want = pending && !bad && lane < upto;
-                const uint32_t eq = __match_any_sync(full_mask, want ? page : ~(uint64_t)lane);
-                const uint32_t leader = __ffs(eq) - 1;
-                uint32_t slot = L.r.acquire_page_warp(full_mask, want && lane == leader, want ? page : 0, __popc(eq), false, vb * 8u);
-                slot = __shfl_sync(full_mask, slot, leader);
+                const uint32_t slot = kv_pin_warp(L, want, page, false, vb * 8u);
                 const bool got = want && slot <= BAM_SLOT_MAX;
                 const uint32_t miss = __ballot_sync(full_mask, want && !got);
                 const uint32_t last = miss ? __ffs(miss) - 1 : upto;               /* the lanes below go out now */
