@@ -318,7 +318,7 @@ extern "C" uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* l
     kv_layout_d_t L;
     if (kv_layout(a, layout, &L) != BAM_OK) return 0;
     const uint32_t most = kv_most_blocks(a);
-    return kv_parts_at(most) + (uint64_t)most * 2 * KV_ROWS * (L.head_dim + 2) * sizeof(float);
+    return kv_parts_at(most * KV_WORKERS) + (uint64_t)most * KV_WORKERS * 2 * KV_ROWS * (L.head_dim + 2) * sizeof(float);
 }
 
 static int check_scratch(bam_array_t a, const bam_kv_layout_t* layout, void* scratch, uint64_t scratch_bytes)

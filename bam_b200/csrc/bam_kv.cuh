@@ -23,6 +23,8 @@
 namespace bam {
 
 #define KV_ROWS 16u                   /* query heads of a unit of the attention: the rows of a matrix instruction */
+#define KV_WORKERS 3u                 /* worker warps of a block of the attention; with the fourth, which only a controller
+                                       * block uses, a thread may have 255 registers */
 
 /* A launch's own words at the head of its scratch, all ones when the launch starts (one memset, so a captured
  * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks.
@@ -185,9 +187,9 @@ int kv_launch(bam_ctrl* c, const Work& work, uint64_t want, void* scratch, size_
     return BAM_OK;
 }
 
-/* Scratch: the launch's words, a counter per worker block, the blocks' parts. */
+/* Scratch: the launch's words, a counter per worker warp of the attention, the workers' parts. */
 inline uint32_t kv_most_blocks(bam_array* a) { return (uint32_t)a->pc->ctrl->num_sms * 2u; }
-inline size_t kv_parts_at(uint32_t blocks) { return (sizeof(kv_launch_words_t) + 4 * (size_t)blocks + 127) / 128 * 128; }
+inline size_t kv_parts_at(uint32_t workers) { return (sizeof(kv_launch_words_t) + 4 * (size_t)workers + 127) / 128 * 128; }
 
 /* The attention's launchers, one translation unit per element type. */
 template <class T>

@@ -12,25 +12,26 @@ namespace bam {
 
 /* The flattened work list: sequence b has `n` chunks of CS tokens with something visible in them, in each of its
  * n_kv_heads * tiles units (a unit: 16 query heads of one key/value head), and the list is b-major, then unit, then
- * chunk.  Worker block i takes the chunks [i * per, (i + 1) * per): every block reads the same amount whatever the
- * lengths are, a long sequence is split over many blocks and a short one is not split at all.  A block that does not
- * own a whole unit writes its running maximum, denominator and unnormalised sum to the scratch; the blocks of a unit
- * wait for each other at the end (they are co-resident, one cooperative launch) and each joins a part of the output,
+ * chunk.  A WARP is a worker: it takes a run of `per` chunks, copies them into its own stages of shared memory and keeps
+ * one running softmax.  Every warp reads the same amount whatever the lengths
+ * are, a long sequence is split over many warps and a short one is not split at all (cuts that fall next to the edge
+ * of a unit move there).  Warps share nothing and wait for nothing of one another until the end: one that does not
+ * own a whole unit writes its running maximum, denominator and unnormalised sum to the scratch, and then the warps of
+ * that unit wait for each other (they are co-resident, one cooperative launch) and each joins a part of the output,
  * adding in a fixed order: the same bits on every run.
  *
  * What bounds it is reading keys and values once from HBM: 4 head_dim bytes a token for 4 head_dim flops a query head,
- * 8 flops a byte at 8 query heads.  So the design feeds bulk copies.  One warp looks pages up and pins them, 32 at a
- * time, up to 64 chunks ahead: a look-up is a chain of six dependent accesses that miss L2 while the rows stream
- * through it, 5 to 10 us.  Three consumer warps take the chunks in turn; each has its own stages of shared memory
- * and refills them itself, keys and values with one bulk copy each, so no warp waits for another between units.  A
- * page is unpinned as soon as its rows have landed.  Every warp keeps one running softmax, merged once per unit.
+ * 8 flops a byte at 8 query heads.  So the design feeds bulk copies: three worker warps a block, two blocks an SM, two or
+ * more chunks under way for each (200 KB of an SM's shared memory).  The fourth warp of a block looks their pages up and
+ * pins them up to 16 chunks ahead: a look-up is three dependent accesses that miss L2 while the rows stream through it,
+ * 2 to 5 us (done by the workers themselves, 32 pages at a time, it cost 10 us of 186 on the largest case).
  * The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured): 16 query heads are
  * all the rows there are, and a chunk of 32 tokens at 128 dimensions takes 200 of the 710 cycles that HBM needs to
  * deliver it to an SM; the 128-row tcgen05 tiles would be seven eighths padding. */
-#define KV_STAGES_MAX 24u
-#define KV_AHEAD 64u                  /* chunks whose pages may be pinned at a time, in batches of 32 */
-#define KV_CONSUMERS 3u               /* consumer warps: with the pinning warp four, which leaves a thread 255 registers */
-#define KV_MIN_CHUNKS 4u              /* a block takes at least so many: below that splitting costs more than it saves */
+#define KV_STAGES_MAX 8u              /* stages of a worker */
+#define KV_AHEAD 16u                  /* chunks of a worker that are pinned and not yet consumed, at most */
+#define KV_PIN_LANES 10u              /* lanes of the pinning warp for each worker */
+#define KV_MIN_CHUNKS 4u              /* a worker takes at least so many: below that splitting costs more than it saves */
 
 struct kv_seen_t {
     int64_t len, first, begin;        /* visible: j < first, and begin <= j < len */
@@ -55,37 +56,35 @@ BAM_DEV void ldm_x4_t(uint32_t (&r)[4], uint32_t addr)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-BAM_DEV void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-template <uint32_t N> BAM_DEV void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N * 32) : "memory"); }
 /* 2^x, off by two units in the last place at most; results below the normal range are 0 */
 BAM_DEV float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-BAM_DEV void st_cg_f4(float* p, float x, float y, float z, float w)
-{
-    asm volatile("st.global.cg.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
-}
 BAM_DEV void st_cg_f2(float* p, float x, float y) { asm volatile("st.global.cg.v2.f32 [%0], {%1,%2};" ::"l"(p), "f"(x), "f"(y) : "memory"); }
-BAM_DEV float ld_cg_f(const float* p) { float v; asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory"); return v; }
+BAM_DEV float2 ld_cg_f2(const float* p) { float2 v; asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory"); return v; }
 
-/* A pinned chunk: where its rows are.  `tag` is 2 r while the place is free for its r-th chunk and 2 r + 1 from the
- * moment that chunk is pinned until it is unpinned. */
-struct kv_pinned_t {
-    uint64_t src;
-    uint32_t slot, rows;              /* rows: first row in the stage << 16 | number of rows; 0: the block was no block */
+/* Where a worker's run begins, or a chunk is: sequence, chunk within the sequence's share of the list. */
+struct kv_place_t {
+    uint64_t f, pos;
+    uint32_t b;
 };
 
-/* Shared memory of a worker block behind its ring of stages. */
-template <int DMAX>
+/* A pinned chunk: where the rows of its pieces are.  `rows`: first row in the stage << 16 | number of rows. */
+struct kv_pinned_t {
+    uint64_t src[2];
+    uint32_t slot[2], rows[2];
+};
+
+/* Shared memory of a worker block behind its stages. */
 struct kv_shared_t {
-    float merge[KV_ROWS][DMAX < 128 ? DMAX : 128];      /* a warp's sums on their way into another's   */
-    float m[KV_CONSUMERS][KV_ROWS], l[KV_CONSUMERS][KV_ROWS];
-    uint64_t full[KV_STAGES_MAX];
-    kv_pinned_t pinned[KV_AHEAD];
-    uint32_t tag[KV_AHEAD];
-    uint64_t warp_sum[8];
-    uint64_t start_pos;
-    uint32_t start_b;
+    uint64_t full[KV_WORKERS][KV_STAGES_MAX];
+    kv_pinned_t pinned[KV_WORKERS][KV_AHEAD];           /* chunk k of a worker at place k % ahead     */
+    uint32_t tag[KV_WORKERS][KV_AHEAD];                 /* 2 r: free for its r-th chunk, 2 r + 1: from then on until that is unpinned */
+    kv_place_t from[KV_WORKERS];                        /* where the workers' runs begin              */
+    uint32_t chunks[KV_WORKERS];                        /* and how long they are                      */
+    uint64_t before[32 * (KV_WORKERS + 1) + 1];         /* chunks of the list before each thread's run of sequences */
+    uint64_t warp_sum[KV_WORKERS + 1];
+    uint32_t warp_max[KV_WORKERS + 1];
     volatile uint32_t abort;
-    struct { uint32_t b, u; uint64_t first; uint32_t n; } join[2];
+    struct { uint32_t b, u; uint64_t first; uint32_t n; } join[KV_WORKERS][2];
 };
 
 BAM_DEV uint32_t ld_acquire_cta(const uint32_t* p) { uint32_t v; asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory"); return v; }
@@ -93,14 +92,12 @@ BAM_DEV void st_release_cta(uint32_t* p, uint32_t v) { asm volatile("st.release.
 
 /* DMAX: the head_dim the registers are laid out for, and with EXACT the head_dim itself (otherwise every step over
  * the dimensions asks whether it is needed, which keeps the compiler from overlapping them: 3 times the time of a
- * chunk at 128); CS: tokens of a chunk (it divides block_tokens). */
+ * chunk at 128); CS: tokens of a chunk. */
 template <class T, int DMAX, int CS, bool EXACT>
 struct KvAttendWork {
-    static constexpr uint32_t CONSUMERS = KV_CONSUMERS;
-    typedef kv_shared_t<DMAX> shared_t;
-    static constexpr int threads = 32 * (CONSUMERS + 1), min_blocks = 2;
+    static constexpr int threads = 32 * (KV_WORKERS + 1), min_blocks = 2;
     static constexpr uint32_t smem = 112 * 1024;
-    static constexpr uint32_t ring_bytes = (smem - 1024u - (uint32_t)sizeof(shared_t)) & ~1023u;
+    static constexpr uint32_t ring_bytes = (smem - 1024u - (uint32_t)sizeof(kv_shared_t)) & ~1023u;
     static constexpr bool pow2_row = EXACT && (DMAX == 64 || DMAX == 128 || DMAX == 256);
     kv_layout_d_t L;
     const uint16_t* q;
@@ -111,22 +108,23 @@ struct KvAttendWork {
     uint32_t batch, n_q_heads, table_width;
     uint32_t q32, o32;                                   /* two elements at a time lie on 4-byte boundaries */
     uint32_t group, tiles;                               /* query heads of a key/value head, units they make */
+    uint32_t ahead;                                      /* KV_AHEAD, or less in a small cache */
+    uint32_t piece;                                      /* tokens of a chunk that are sure to lie in one page: CS or 16 */
     float scale_log2;                                    /* its magnitude; the sign goes into the query */
     uint32_t q_sign;
     int64_t window, sinks;
-    uint32_t* arrived;                                   /* per worker block, all ones at the start: arrivals at the unit it begins */
-    float* parts;                                        /* [worker block][2]: head_dim x 16 sums, 16 maxima, 16 denominators */
+    uint32_t* arrived;                                   /* per worker, all ones at the start: arrivals at the unit it begins */
+    float* parts;                                        /* [worker][2]: rows x head_dim sums, 16 maxima, 16 denominators */
 
     BAM_DEV uint32_t dim() const { return EXACT ? (uint32_t)DMAX : L.head_dim; }
     BAM_DEV uint32_t row_bytes() const { return dim() * 2u; }
+    BAM_DEV uint32_t stage_bytes() const { return CS * dim() * 4u; }
     BAM_DEV uint32_t stages() const
     {
-        /* a multiple of the consumers: every stage then belongs to one warp, which meets its uses in order (a phase
-         * of an mbarrier can only be told from the one before it) */
-        const uint32_t n = ring_bytes / (CS * dim() * 4u);
-        return (n < KV_STAGES_MAX ? n : KV_STAGES_MAX) / CONSUMERS * CONSUMERS;
+        const uint32_t n = ring_bytes / (KV_WORKERS * stage_bytes());
+        return n < KV_STAGES_MAX ? n : KV_STAGES_MAX;
     }
-    BAM_DEV float* part(uint32_t block, uint32_t which) const { return parts + ((size_t)block * 2 + which) * (KV_ROWS * (dim() + 2)); }
+    BAM_DEV float* part(uint32_t worker, uint32_t which) const { return parts + ((size_t)worker * 2 + which) * (KV_ROWS * (dim() + 2)); }
 
     BAM_DEV kv_seen_t seen(uint32_t b, bool tell = false) const
     {
@@ -151,10 +149,65 @@ struct KvAttendWork {
     }
     BAM_DEV static int64_t first_token(const kv_seen_t& v, uint32_t c) { return (int64_t)(c < v.n_first ? c : v.from + (c - v.n_first)) * CS; }
 
+    /* ---- the list ------------------------------------------------------------------------------------- */
+    /* how far a cut between two workers moves to fall on the edge of a unit: a join costs what two chunks do */
+    BAM_DEV static uint64_t slack(uint64_t per) { return per / 4 < 2 ? per / 4 : 2; }
+
+    /* The cut before worker i: chunk i * per, or the edge of its unit if that is near.  All lanes. */
+    BAM_DEV kv_place_t cut(const kv_shared_t& sh, uint64_t i, uint64_t per, uint64_t total) const
+    {
+        const uint32_t lane = lane_id(), units = L.n_kv_heads * tiles;
+        const uint64_t x = i * per;
+        kv_place_t p = { total, 0, 0 };
+        if (x >= total) return p;
+        uint32_t t = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < KV_WORKERS + 1; k++) t += __popc(__ballot_sync(0xffffffffu, sh.before[k * 32 + lane] <= x));
+        t -= 1;
+        const uint32_t run = (batch + threads - 1) / threads;
+        uint64_t at = sh.before[t];
+        for (uint32_t b0 = t * run;; b0 += 32) {                    /* the sequence in the thread's run */
+            const uint32_t b = b0 + lane;
+            uint64_t span = b < batch && b < (t + 1) * run ? (uint64_t)seen(b).n * units : 0u, upto = span;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += y;
+            }
+            const uint32_t m = __ballot_sync(0xffffffffu, x < at + upto);
+            if (m == 0u) {
+                at += __shfl_sync(0xffffffffu, upto, 31);
+                if (b0 + 32 >= (t + 1) * run) return p;             /* the lengths changed under the launch */
+                continue;
+            }
+            const uint32_t src = __ffs(m) - 1;
+            p.b = b0 + src;
+            at += __shfl_sync(0xffffffffu, upto - span, src);
+            break;
+        }
+        const uint64_t n = seen(p.b).n, in = (x - at) % n;
+        p.f = x;
+        if (in <= slack(per)) p.f = x - in;
+        else if (n - in <= slack(per)) p.f = x + (n - in);
+        p.pos = p.f - at;
+        return p;
+    }
+    /* the first worker of the unit [U0, U1), and how many there are (see cut) */
+    BAM_DEV static void workers_of(uint64_t U0, uint64_t U1, uint64_t per, uint32_t& first, uint32_t& count)
+    {
+        uint64_t i0 = U0 / per, i1 = (U1 - 1) / per;
+        const uint64_t up = (i0 + 1) * per, down = i1 * per;
+        if (up < U1 && up - U0 <= slack(per)) i0++;
+        if (down > U0 && down - U0 > slack(per) && U1 - down <= slack(per)) i1--;
+        first = (uint32_t)i0;
+        count = (uint32_t)(i1 - i0 + 1);
+    }
+
+    /* ---- pages and copies ----------------------------------------------------------------------------- */
     /* A warp's wait, and it ends: `done`, asked by all lanes together, says when; false when the block gives up
      * (someone's wait ran out, or the status block says so). */
     template <class Done>
-    BAM_DEV bool wait(shared_t& sh, Done done) const
+    BAM_DEV bool wait(kv_shared_t& sh, Done done) const
     {
         uint32_t polls = 0;
         uint64_t t0 = 0;
@@ -164,7 +217,7 @@ struct KvAttendWork {
                 bam_status_t* st = L.r.cache.status;
                 const uint64_t now = global_timer_ns();
                 if (t0 == 0) t0 = now;
-                /* the pinning warp's own waits have one limit each; twice that is more than it needs to report */
+                /* the waits inside an acquire have one limit each; twice that is more than it needs to report */
                 if (now - t0 > 2 * st->spin_timeout_ns) status_fail(st, BAM_ETIMEDOUT, BAM_AT_TMA, polls);
                 stop |= status_bad(st);
             }
@@ -173,145 +226,172 @@ struct KvAttendWork {
         return true;
     }
 
-    /* ---- the pinning warp ------------------------------------------------------------------------------ */
-    BAM_DEV void pin_ahead(shared_t& sh, uint64_t f0, uint64_t f1, uint32_t vb) const
+    /* The pinning warp: KV_PIN_LANES lanes work for each worker, one page each. */
+    BAM_DEV void pin_ahead(kv_shared_t& sh, uint32_t vb) const
     {
-        const uint32_t full_mask = 0xffffffffu, lane = lane_id();
-        const uint32_t units = L.n_kv_heads * tiles;
-        uint32_t base_b = sh.start_b;
-        uint64_t base_pos = sh.start_pos;
+        const uint32_t full_mask = 0xffffffffu, lane = lane_id(), pieces = CS / piece, units = L.n_kv_heads * tiles;
+        const bool works = lane < KV_WORKERS * KV_PIN_LANES;
+        const uint32_t w = works ? lane / KV_PIN_LANES : 0, i = lane - w * KV_PIN_LANES, c = i / pieces, k = i - c * pieces;
+        const uint32_t mask = ((1u << KV_PIN_LANES) - 1u) << (w * KV_PIN_LANES);       /* the lanes of my worker */
+        const uint32_t most = KV_PIN_LANES / pieces < ahead ? KV_PIN_LANES / pieces : ahead;
+        const uint32_t end = works ? sh.chunks[w] : 0;
+        kv_place_t at = sh.from[w];                       /* where chunk `next` of the worker is */
+        uint32_t next = 0, ask = most;                    /* chunks asked for at a time: fewer in a cache that is too full for all */
         spin_t sp;
-        for (uint64_t f = f0; f < f1; f += 32) {
-            bool pending = f + lane < f1;
-            /* where this lane's chunk is */
-            uint32_t b = base_b, rows = 0;
-            uint64_t pos = base_pos + lane, page = 0, offset = 0;
-            bool bad = false;
-            if (pending) {
+        for (;;) {
+            const uint32_t n = next + c, round = n / ahead, place = n - round * ahead;
+            bool mine = false;
+            /* the next chunks that have a place */
+            if (!wait(sh, [&] {
+                    mine = n < end && c < ask && ld_acquire_cta(&sh.tag[w][place]) == 2u * round;
+                    return __any_sync(full_mask, mine) || __all_sync(full_mask, next >= end);
+                })) return;
+            if (!__any_sync(full_mask, mine)) return;     /* all runs are pinned */
+            const uint32_t gap = ~__ballot_sync(full_mask, mine) & mask;                 /* (the places come free in order) */
+            if (gap && lane > (uint32_t)__ffs(gap) - 1u) mine = false;
+            uint32_t b = at.b, rows = 0, slot = BAM_SLOT_NONE;
+            uint64_t pos = at.pos + c, page = 0, offset = 0;
+            bool want = false;
+            if (mine) {
                 kv_seen_t v = seen(b);
                 while (pos >= (uint64_t)v.n * units && b + 1 < batch) { pos -= (uint64_t)v.n * units; v = seen(++b); }
-                if (v.n == 0) { sh.abort = 1; v.n = 1; }                   /* the lengths changed under the launch */
-                const uint32_t u = (uint32_t)(pos / v.n), c = (uint32_t)(pos - (uint64_t)u * v.n);
-                const int64_t t0 = first_token(v, c);
-                int64_t lo = t0, hi = t0 + CS < v.len ? t0 + CS : v.len;
-                if (t0 >= v.first && lo < v.begin) lo = v.begin;
-                if (t0 + CS <= v.begin && hi > v.first) hi = v.first;
-                const int64_t block = __ldg(table + b * table_stride + t0 / L.block_tokens);
-                bad = block < 0 || (uint64_t)block >= L.n_blocks;
-                if (bad) L.bad_index((uint64_t)block);
-                else {
-                    page = L.page_of((uint64_t)block, u / tiles);
-                    rows = (uint32_t)(lo - t0) << 16 | (uint32_t)(hi - lo);
-                    offset = (uint64_t)(lo % L.block_tokens) * row_bytes();
+                if (v.n == 0) { sh.abort = 1; v.n = 1; }                                 /* the lengths changed under the launch */
+                const uint32_t u = (uint32_t)(pos / v.n), ci = (uint32_t)(pos - (uint64_t)u * v.n);
+                const int64_t t0 = first_token(v, ci), tb = t0 + k * piece;
+                int64_t lo = tb, hi = tb + piece < v.len ? tb + piece : v.len;
+                if (tb >= v.first && lo < v.begin) lo = v.begin;
+                if (tb + piece <= v.begin && hi > v.first) hi = v.first;
+                if (lo < hi) {
+                    const int64_t block = __ldg(table + b * table_stride + tb / L.block_tokens);
+                    if (block < 0 || (uint64_t)block >= L.n_blocks) L.bad_index((uint64_t)block);
+                    else {
+                        want = true;
+                        page = L.page_of((uint64_t)block, u / tiles);
+                        rows = (uint32_t)(lo - t0) << 16 | (uint32_t)(hi - lo);
+                        offset = (uint64_t)(lo % L.block_tokens) * row_bytes();
+                    }
                 }
             }
-            base_b = __shfl_sync(full_mask, b, 31);
-            base_pos = __shfl_sync(full_mask, pos, 31) + 1;
-            const uint32_t k = (uint32_t)(f - f0) + lane, place = k % KV_AHEAD, round = k / KV_AHEAD;
-            if (!wait(sh, [&] { return __all_sync(full_mask, !pending || ld_acquire_cta(&sh.tag[place]) == 2u * round); })) return;
-            /* A lane whose page cannot be had now is asked for again when
-             * the chunks before it have been handed on, and the chunks behind it give theirs back meanwhile: what a
-             * block holds is always the next it needs, so blocks never wait for pages that wait for them */
-            sp.reset();
-            uint32_t ask = 32;                 /* lanes that ask at a time: fewer in a cache that is too full for all, down to one */
-            for (;;) {
-                const uint32_t todo = __ballot_sync(full_mask, pending);
-                if (todo == 0u) break;
-                const uint32_t upto = __ffs(todo) - 1 + ask;
-                const bool want = pending && !bad && lane < upto;
-                const uint32_t slot = kv_pin_warp(L, want, page, false, vb * 8u);
-                const bool got = want && slot <= BAM_SLOT_MAX;
-                const uint32_t miss = __ballot_sync(full_mask, want && !got);
-                const uint32_t last = miss ? __ffs(miss) - 1 : upto;               /* the lanes below go out now */
-                ask = miss ? (ask + 1) / 2 : (ask < 32u ? ask * 2 : 32u);
-                const bool failed = __any_sync(full_mask, want && slot == BAM_SLOT_ERR);
-                if (got && (lane >= last || failed)) L.r.release_page(slot, 1);
-                if (failed) { sh.abort = 1; return; }
-                if (pending && lane < last) {
-                    kv_pinned_t* e = &sh.pinned[place];
-                    e->src = got ? L.r.get_cache_page_addr(slot) + offset : 0;
-                    e->slot = got ? slot : BAM_SLOT_NONE;
-                    e->rows = rows;
-                    st_release_cta(&sh.tag[place], 2u * round + 1u);
-                    pending = false;
-                }
-                if (__ballot_sync(full_mask, pending) == todo && __any_sync(full_mask, sp.expired(L.r.cache.status, BAM_AT_FIND_SLOT, page))) {
-                    sh.abort = 1;
-                    return;
-                }
+            slot = kv_pin_warp(L, want, page, false, vb * KV_WORKERS);
+            const bool got = want && slot <= BAM_SLOT_MAX;
+            const bool failed = __any_sync(full_mask, want && slot == BAM_SLOT_ERR);
+            /* What could not be had is asked for again; the chunks of the worker behind it give theirs back meanwhile, and
+             * those before it are handed on.  So what a block holds pinned is always what its workers consume without
+             * anybody's help, and blocks never wait for pages that wait for them. */
+            const uint32_t miss = __ballot_sync(full_mask, want && !got) & mask, taken = __ballot_sync(full_mask, mine) & mask;
+            const uint32_t ready = (miss ? __ffs(miss) - 1u - w * KV_PIN_LANES : (uint32_t)__popc(taken)) / pieces;     /* chunks */
+            if (got && (c >= ready || failed)) L.r.release_page(slot, 1);
+            if (failed) { sh.abort = 1; return; }
+            if (mine && c < ready) {
+                kv_pinned_t* e = &sh.pinned[w][place];
+                e->src[k] = got ? L.r.get_cache_page_addr(slot) + offset : 0;
+                e->slot[k] = got ? slot : BAM_SLOT_NONE;
+                e->rows[k] = got ? rows : 0;
             }
+            __syncwarp();
+            if (mine && c < ready && k == 0) st_release_cta(&sh.tag[w][place], 2u * round + 1u);
+            const uint32_t last = w * KV_PIN_LANES + (ready ? ready * pieces - 1 : 0);
+            const uint32_t lb = __shfl_sync(full_mask, b, last);
+            const uint64_t lpos = __shfl_sync(full_mask, pos, last);
+            if (ready) { next += ready; at.b = lb; at.pos = lpos + 1; }
+            ask = miss ? (ask + 1) / 2 : (ask * 2 < most ? ask * 2 : most);
+            if (!__any_sync(full_mask, ready)) {
+                if (__any_sync(full_mask, sp.expired(L.r.cache.status, BAM_AT_FIND_SLOT, page))) { sh.abort = 1; return; }
+            } else sp.reset();
         }
     }
 
-    /* ---- consumers ----------------------------------------------------------------------------------- */
-    BAM_DEV uint32_t q_pair(const uint16_t* row, uint32_t d) const
-    {
-        if (q32) return __ldg(reinterpret_cast<const uint32_t*>(row + d));
-        return (uint32_t)__ldg(row + d) | ((uint32_t)__ldg(row + d + 1) << 16);
-    }
-    /* the query fragment of dimensions [16 ks, 16 ks + 16): rows lane / 4 and lane / 4 + 8 */
-    BAM_DEV void load_q(uint32_t (&a)[4], const uint16_t* r0, const uint16_t* r1, uint32_t ks) const
-    {
-        const uint32_t d = ks * 16 + (lane_id() & 3u) * 2;
-        a[0] = r0 ? q_pair(r0, d) ^ q_sign : 0u;
-        a[1] = r1 ? q_pair(r1, d) ^ q_sign : 0u;
-        a[2] = r0 ? q_pair(r0, d + 8) ^ q_sign : 0u;
-        a[3] = r1 ? q_pair(r1, d + 8) ^ q_sign : 0u;
-    }
-
-    /* A consumer warp's own chunks of the block (w, w + CONSUMERS, ...) and its stages. */
-    struct ring_t {
-        uint32_t base, end;             /* shared address of the ring; chunks of the block                */
-        uint32_t next, stage, use;      /* the chunk that is consumed next, its stage and how often that was used */
+    /* A worker's pipeline. */
+    struct pipe_t {
+        uint32_t base, w;               /* shared address of the worker's stages; its number in the block */
+        uint32_t end;                   /* chunks of the run                                              */
+        uint32_t next, stage, use;      /* the chunk that is consumed next, its stage and how often that was used before */
+        uint32_t next_place, next_round;
         uint32_t issue, issue_stage;    /* the chunk that is copied next                                  */
+        uint32_t issue_place, issue_round;
     };
 
-    /* Start the copies of the warp's next chunk, if it has a free stage and the chunk is pinned; false if not.  Nothing
-     * is waited for: what the warp holds pinned is what it consumes without anybody's help, so that blocks never wait
-     * for pages that wait for them. */
-    BAM_DEV bool issue_next(shared_t& sh, ring_t& g) const
+    /* Start the copies of the worker's next chunk, if it has a free stage and the chunk is pinned; false if not. */
+    BAM_DEV bool issue_next(kv_shared_t& sh, pipe_t& g) const
     {
         if (g.issue >= g.end || g.issue - g.next >= stages()) return false;
-        const uint32_t place = g.issue % KV_AHEAD, round = g.issue / KV_AHEAD;
-        uint32_t ready = 0;
-        if (lane_id() == 0) ready = ld_acquire_cta(&sh.tag[place]) == 2u * round + 1u ? 1u : 0u;
-        if (!__shfl_sync(0xffffffffu, ready, 0)) return false;
-        if (lane_id() == 0) {
-            const kv_pinned_t e = sh.pinned[place];
-            const uint32_t full = smem_u32(&sh.full[g.issue_stage]);
-            if (e.slot == BAM_SLOT_NONE) mbar_arrive(full);
-            else {
-                const uint32_t bytes = (e.rows & 0xffffu) * row_bytes();
-                const uint32_t dst = g.base + g.issue_stage * (CS * dim() * 4u) + (e.rows >> 16) * row_bytes();
-                /* pages that this launch fetched were written by bulk copies too; order those before ours */
-                asm volatile("fence.proxy.async.global;" ::: "memory");
-                mbar_expect_tx(full, 2 * bytes);
-                bulk_load(dst, reinterpret_cast<const void*>(e.src), bytes, full);
-                bulk_load(dst + CS * row_bytes(), reinterpret_cast<const void*>(e.src + L.v_offset()), bytes, full);
+        const uint32_t lane = lane_id();
+        if (!__all_sync(0xffffffffu, ld_acquire_cta(&sh.tag[g.w][g.issue_place]) == 2u * g.issue_round + 1u)) return false;
+        if (lane == 0) {
+            const kv_pinned_t e = sh.pinned[g.w][g.issue_place];
+            const uint32_t full = smem_u32(&sh.full[g.w][g.issue_stage]), dst = g.base + g.issue_stage * stage_bytes();
+            const uint32_t n0 = (e.rows[0] & 0xffffu) * row_bytes(), n1 = piece < CS ? (e.rows[1] & 0xffffu) * row_bytes() : 0;
+            /* pages that this launch fetched were written by bulk copies too; order those before ours */
+            asm volatile("fence.proxy.async.global;" ::: "memory");
+            mbar_expect_tx(full, 2 * (n0 + n1));
+            if (n0) {
+                const uint32_t d = dst + (e.rows[0] >> 16) * row_bytes();
+                bulk_load(d, reinterpret_cast<const void*>(e.src[0]), n0, full);
+                bulk_load(d + CS * row_bytes(), reinterpret_cast<const void*>(e.src[0] + L.v_offset()), n0, full);
+            }
+            if (n1) {
+                const uint32_t d = dst + (e.rows[1] >> 16) * row_bytes();
+                bulk_load(d, reinterpret_cast<const void*>(e.src[1]), n1, full);
+                bulk_load(d + CS * row_bytes(), reinterpret_cast<const void*>(e.src[1] + L.v_offset()), n1, full);
             }
         }
         __syncwarp();
-        g.issue += CONSUMERS;
-        g.issue_stage += CONSUMERS;
-        if (g.issue_stage >= stages()) g.issue_stage -= stages();
+        g.issue++;
+        if (++g.issue_stage == stages()) g.issue_stage = 0;
+        if (++g.issue_place == ahead) { g.issue_place = 0; g.issue_round++; }
         return true;
     }
-    /* Wait until the warp's next chunk has landed, and start copies of later ones meanwhile. */
-    BAM_DEV bool landed(shared_t& sh, ring_t& g) const
+
+    /* Wait until the next chunk has landed, and start copies of later ones meanwhile. */
+    BAM_DEV bool landed(kv_shared_t& sh, pipe_t& g) const
     {
-        const uint32_t full = smem_u32(&sh.full[g.stage]);
+        const uint32_t full = smem_u32(&sh.full[g.w][g.stage]);
         return wait(sh, [&] {
             while (issue_next(sh, g)) {}
             return g.next < g.issue && __all_sync(0xffffffffu, mbar_test(full, g.use & 1u));
         });
     }
-    /* The warp's next chunk has landed: unpin its page.  (Lane 0.)  The rows are in shared memory, nothing of this
-     * thread is outstanding that a release would have to wait for; its fence held the warp up for 2000 cycles. */
-    BAM_DEV void unpin(shared_t& sh, uint32_t n) const
+    /* The next chunk has landed: unpin its pages.  The rows are in shared memory, nothing of this thread is outstanding
+     * that a release would have to wait for; its fence held the warp up for 2000 cycles a chunk. */
+    BAM_DEV void unpin(kv_shared_t& sh, const pipe_t& g) const
     {
-        const uint32_t place = n % KV_AHEAD, slot = sh.pinned[place].slot;
-        if (slot != BAM_SLOT_NONE) red_add_relaxed(&L.r.cache.slots[slot].state, 0u - 1u);
-        st_release_cta(&sh.tag[place], 2u * (n / KV_AHEAD) + 2u);
+        const uint32_t lane = lane_id();
+        if (lane < CS / piece) {
+            const uint32_t slot = sh.pinned[g.w][g.next_place].slot[lane];
+            if (slot != BAM_SLOT_NONE) red_add_relaxed(&L.r.cache.slots[slot].state, 0u - 1u);
+        }
+        __syncwarp();
+        if (lane == 0) st_release_cta(&sh.tag[g.w][g.next_place], 2u * g.next_round + 2u);
+    }
+    BAM_DEV void advance(pipe_t& g) const
+    {
+        g.next++;
+        if (++g.stage == stages()) { g.stage = 0; g.use++; }
+        if (++g.next_place == ahead) { g.next_place = 0; g.next_round++; }
+    }
+
+    /* ---- products ------------------------------------------------------------------------------------- */
+    /* the query fragments: rows lane / 4 and lane / 4 + 8 of the unit, head_dim in steps of 16 */
+    BAM_DEV void load_q(uint32_t (&a)[DMAX / 16][4], const uint16_t* r0, const uint16_t* r1) const
+    {
+        const uint32_t d0 = (lane_id() & 3u) * 2;
+        if (q32) {
+#pragma unroll
+            for (int i = 0; i < DMAX / 4; i++) {
+                const uint16_t* r = i & 1 ? r1 : r0;
+                const uint32_t d = (i >> 2) * 16 + d0 + (i & 2) * 4;
+                a[i >> 2][i & 3] = r && (EXACT || (i >> 2) * 16 < (int)L.head_dim) ? __ldg(reinterpret_cast<const uint32_t*>(r + d)) : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < DMAX / 4; i++) {
+                const uint16_t* r = i & 1 ? r1 : r0;
+                const uint32_t d = (i >> 2) * 16 + d0 + (i & 2) * 4;
+                a[i >> 2][i & 3] = r && (EXACT || (i >> 2) * 16 < (int)L.head_dim) ? (uint32_t)__ldg(r + d) | ((uint32_t)__ldg(r + d + 1) << 16) : 0u;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DMAX / 4; i++) a[i >> 2][i & 3] ^= q_sign;
     }
 
     struct state_t {
@@ -448,81 +528,41 @@ struct KvAttendWork {
             }
         }
     }
-    BAM_DEV void write_part(const state_t& z, float* p) const
+    /* query heads of unit u */
+    BAM_DEV uint32_t rows_of(uint32_t u) const
+    {
+        const uint32_t r0 = u % tiles * KV_ROWS;
+        return group - r0 < KV_ROWS ? group - r0 : KV_ROWS;
+    }
+    BAM_DEV void write_part(const state_t& z, float* p, uint32_t rows) const
     {
         const uint32_t lane = lane_id();
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint32_t r = (lane >> 2) + 8 * half;
-            float* row = p + r * dim() + (lane & 3u) * 2;
+            if (r < rows) {
+                float* row = p + r * dim() + (lane & 3u) * 2;
 #pragma unroll
-            for (int i = 0; i < DMAX / 8; i++)
-                if (i * 8 < (int)L.head_dim || EXACT) st_cg_f2(row + i * 8, z.o[i][2 * half], z.o[i][2 * half + 1]);
-            if ((lane & 3u) == 0u) {
-                float* ml = p + KV_ROWS * dim();
-                ml[r] = z.m[half];
-                ml[KV_ROWS + r] = z.l[half];
+                for (int i = 0; i < DMAX / 8; i++)
+                    if (EXACT || i * 8 < (int)L.head_dim) st_cg_f2(row + i * 8, z.o[i][2 * half], z.o[i][2 * half + 1]);
+                if ((lane & 3u) == 0u) st_cg_f2(p + KV_ROWS * dim() + 2 * r, z.m[half], z.l[half]);
             }
         }
     }
 
-    /* Merge the consumers' states into warp 0's. */
-    BAM_DEV void merge(shared_t& sh, state_t& z, uint32_t w) const
+    /* ---- a worker ------------------------------------------------------------------------------------- */
+    BAM_DEV void work(kv_shared_t& sh, uint32_t ring, uint64_t per, uint32_t worker) const
     {
-        const uint32_t lane = lane_id(), row = lane >> 2;
-        if ((lane & 3u) == 0u) {
-#pragma unroll
-            for (int half = 0; half < 2; half++) { sh.m[w][row + 8 * half] = z.m[half]; sh.l[w][row + 8 * half] = z.l[half]; }
-        }
-        consumers_sync<CONSUMERS>();
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const uint32_t r = row + 8 * half;
-            float M = -INFINITY, l = 0.f;
-#pragma unroll
-            for (uint32_t k = 0; k < CONSUMERS; k++) M = fmaxf(M, sh.m[k][r]);
-            const float c = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (uint32_t k = 0; k < CONSUMERS; k++) l += sh.l[k][r] * exp2_fast(sh.m[k][r] - c);
-            const float a = exp2_fast(z.m[half] - c);
-            z.m[half] = M;
-            z.l[half] = l;
-#pragma unroll
-            for (int i = 0; i < DMAX / 8; i++) { z.o[i][2 * half] *= a; z.o[i][2 * half + 1] *= a; }
-        }
-        /* warp 2's sums into warp 1's, those into warp 0's, through one buffer of up to 128 dimensions at a time */
-        constexpr int W = DMAX < 128 ? DMAX : 128;
-#pragma unroll
-        for (int d0 = 0; d0 < DMAX; d0 += W) {
-            auto move = [&](bool in) {
-#pragma unroll
-                for (int i = d0 / 8; i < (d0 + W) / 8; i++) {
-                    if (i * 8 < DMAX && (EXACT || i * 8 < (int)L.head_dim)) {
-                        float2* p = reinterpret_cast<float2*>(&sh.merge[row][i * 8 - d0 + (lane & 3u) * 2]);
-                        float2* q8 = reinterpret_cast<float2*>(&sh.merge[row + 8][i * 8 - d0 + (lane & 3u) * 2]);
-                        if (in) { z.o[i][0] += p->x; z.o[i][1] += p->y; z.o[i][2] += q8->x; z.o[i][3] += q8->y; }
-                        else { *p = make_float2(z.o[i][0], z.o[i][1]); *q8 = make_float2(z.o[i][2], z.o[i][3]); }
-                    }
-                }
-            };
-            static_assert(CONSUMERS == 3, "the chain below");
-            if (w == 2) move(false);
-            consumers_sync<CONSUMERS>();
-            if (w == 1) { move(true); move(false); }          /* a thread writes where it has read */
-            consumers_sync<CONSUMERS>();
-            if (w == 0) move(true);
-            consumers_sync<CONSUMERS>();
-        }
-    }
-
-    BAM_DEV void consume(shared_t& sh, uint32_t ring, uint64_t f0, uint64_t f1, uint64_t per, uint32_t vb) const
-    {
-        const uint32_t lane = lane_id(), w = threadIdx.x >> 5;
-        const uint32_t S = stages(), stage_bytes = CS * dim() * 4u, units = L.n_kv_heads * tiles;
-        uint32_t b = sh.start_b, n_join = 0;
-        uint64_t pos = sh.start_pos;
-        ring_t g = { ring, (uint32_t)(f1 - f0), w, w, 0, w, w };
-        for (uint64_t f = f0; f < f1;) {
+        const uint32_t lane = lane_id(), w = threadIdx.x >> 5, units = L.n_kv_heads * tiles;
+        pipe_t g;
+        g.base = ring + w * stages() * stage_bytes(); g.w = w;
+        const kv_place_t from = sh.from[w];
+        g.end = sh.chunks[w];
+        g.next = g.stage = g.use = g.issue = g.issue_stage = g.next_place = g.next_round = g.issue_place = g.issue_round = 0;
+        const uint64_t f1 = from.f + g.end;
+        uint32_t b = from.b, n_join = 0;
+        uint64_t pos = from.pos;
+        for (uint64_t f = from.f; f < f1;) {
             const kv_seen_t v = seen(b);
             if (pos >= (uint64_t)v.n * units) {
                 pos -= (uint64_t)v.n * units;
@@ -540,114 +580,155 @@ struct KvAttendWork {
             z.m[0] = z.m[1] = -INFINITY;
             z.l[0] = z.l[1] = 0.f;
             uint32_t qa[DMAX / 16][4];
-            const uint32_t mine = (w + CONSUMERS - (uint32_t)((f - f0) % CONSUMERS)) % CONSUMERS;      /* first chunk of the segment that is this warp's */
-            if (mine < seg) {
-#pragma unroll
-                for (int ks = 0; ks < DMAX / 16; ks++)
-                    if (EXACT || ks * 16 < (int)L.head_dim) load_q(qa[ks], q0, q1, ks);
-            }
-            for (uint32_t i = mine; i < seg; i += CONSUMERS) {
-                if (!landed(sh, g)) continue;
-                const bool there = sh.pinned[g.next % KV_AHEAD].slot != BAM_SLOT_NONE;
+            load_q(qa, q0, q1);
+            for (uint32_t i = 0; i < seg; i++) {
+                if (!landed(sh, g)) break;
+                unpin(sh, g);
+                const uint32_t stage = g.base + g.stage * stage_bytes();
+                const int64_t t0 = first_token(v, c + i);
+                if (t0 + CS <= v.first || (t0 >= v.begin && t0 + CS <= v.len)) chunk<true>(z, qa, stage, v, t0);
+                else chunk<false>(z, qa, stage, v, t0);
                 __syncwarp();
-                if (lane == 0) unpin(sh, g.next);
-                if (there) {
-                    const int64_t t0 = first_token(v, c + i);
-                    if (t0 + CS <= v.first || (t0 >= v.begin && t0 + CS <= v.len)) chunk<true>(z, qa, ring + g.stage * stage_bytes, v, t0);
-                    else chunk<false>(z, qa, ring + g.stage * stage_bytes, v, t0);
-                }
-                __syncwarp();
-                g.next += CONSUMERS;
-                g.stage += CONSUMERS;
-                if (g.stage >= S) { g.stage -= S; g.use++; }
+                advance(g);
             }
+            if (__any_sync(0xffffffffu, sh.abort)) break;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 z.l[half] += __shfl_xor_sync(0xffffffffu, z.l[half], 1);
                 z.l[half] += __shfl_xor_sync(0xffffffffu, z.l[half], 2);
             }
-            if (seg > 1) merge(sh, z, w);
-            const bool holds = seg > 1 ? w == 0 : mine == 0;
-            if (seg == v.n) {
-                if (holds) write_out(z, b, u);
-            } else {
+            if (seg == v.n) write_out(z, b, u);
+            else {
                 const uint64_t U0 = f - c;
-                const uint32_t i0 = (uint32_t)(U0 / per);
-                if (holds) {
-                    write_part(z, part(vb, vb == i0 ? 1 : 0));
-                    __threadfence();
-                    __syncwarp();
-                    if (lane == 0 && !sh.abort) (void)atom_add_acq_rel(arrived + i0, 1u);
-                    if (lane == 0) { sh.join[n_join].b = b; sh.join[n_join].u = u; sh.join[n_join].first = U0; sh.join[n_join].n = v.n; }
+                uint32_t i0, cnt;
+                workers_of(U0, U0 + v.n, per, i0, cnt);
+                write_part(z, part(worker, worker == i0 ? 1 : 0), rows_of(u));
+                __threadfence();
+                __syncwarp();
+                if (lane == 0) {
+                    (void)atom_add_acq_rel(arrived + i0, 1u);
+                    sh.join[w][n_join].b = b; sh.join[w][n_join].u = u; sh.join[w][n_join].first = U0; sh.join[w][n_join].n = v.n;
                 }
                 n_join++;
             }
             f += seg;
             pos += seg;
         }
-        /* given up: copies that are still under way land (bounded) before the block leaves */
-        while (g.next < g.issue) {
-            const uint64_t since = global_timer_ns();
-            const uint32_t full = smem_u32(&sh.full[g.stage]);
-            while (!mbar_test(full, g.use & 1u) && global_timer_ns() - since < 2 * L.r.cache.status->spin_timeout_ns) {}
-            __syncwarp();
-            if (lane == 0) unpin(sh, g.next);
-            g.next += CONSUMERS;
-            g.stage += CONSUMERS;
-            if (g.stage >= S) { g.stage -= S; g.use++; }
+        if (g.next < g.end) {
+            /* given up: copies that are still under way land (bounded) before the block leaves */
+            while (g.next < g.issue) {
+                const uint64_t since = global_timer_ns();
+                const uint32_t full = smem_u32(&sh.full[w][g.stage]);
+                while (!mbar_test(full, g.use & 1u) && global_timer_ns() - since < 2 * L.r.cache.status->spin_timeout_ns) {}
+                __syncwarp();
+                unpin(sh, g);
+                advance(g);
+            }
+            return;
         }
-        consumers_sync<CONSUMERS>();
-        for (uint32_t k = 0; k < n_join; k++) join(sh, sh.join[k].b, sh.join[k].u, sh.join[k].first, sh.join[k].n, per, vb);
+        __syncwarp();
+        for (uint32_t k = 0; k < n_join; k++) join(sh, sh.join[w][k].b, sh.join[w][k].u, sh.join[w][k].first, sh.join[w][k].n, per, worker);
     }
 
-    /* This block's share of a unit that several blocks worked on. */
-    BAM_DEV void join(shared_t& sh, uint32_t b, uint32_t u, uint64_t U0, uint32_t n, uint64_t per, uint32_t vb) const
+    /* This worker's share of a unit that several worked on. */
+    BAM_DEV void join(kv_shared_t& sh, uint32_t b, uint32_t u, uint64_t U0, uint32_t n, uint64_t per, uint32_t worker) const
     {
-        const uint32_t lane = lane_id(), w = threadIdx.x >> 5, D = dim();
-        const uint32_t i0 = (uint32_t)(U0 / per), cnt = (uint32_t)((U0 + n - 1) / per) - i0 + 1, j = vb - i0;
-        if (threadIdx.x == 0) {
-            spin_t sp;
-            while (ld_acquire_gpu(arrived + i0) != cnt - 1u) {
-                if (sh.abort) break;
-                if (sp.expired(L.r.cache.status, BAM_AT_KV_JOIN, i0)) { sh.abort = 1; break; }
+        const uint32_t lane = lane_id(), D = dim();
+        uint32_t i0, cnt;
+        workers_of(U0, U0 + n, per, i0, cnt);
+        bam_status_t* st = L.r.cache.status;
+        uint32_t polls = 0, gone = 0;
+        uint64_t t0 = 0;
+        if (lane == 0) {
+            while (ld_acquire_gpu(arrived + i0) != cnt - 1u && !gone) {
+                if (((++polls) & 63u) == 0u) {
+                    const uint64_t now = global_timer_ns();
+                    if (t0 == 0) t0 = now;
+                    if (now - t0 > st->spin_timeout_ns) status_fail(st, BAM_ETIMEDOUT, BAM_AT_KV_JOIN, i0);
+                    gone = status_bad(st) ? 1u : 0u;
+                }
             }
         }
-        consumers_sync<CONSUMERS>();
-        if (__any_sync(0xffffffffu, sh.abort)) return;
+        if (__shfl_sync(0xffffffffu, gone, 0)) return;
         const uint32_t h = u / tiles, r0 = (u - h * tiles) * KV_ROWS;
-        const uint32_t rows = group - r0 < KV_ROWS ? group - r0 : KV_ROWS, quads = rows * (D / 4);
+        const uint32_t quads = rows_of(u) * (D / 4), j = worker - i0;
         const uint32_t g0 = (uint32_t)((uint64_t)quads * j / cnt), g1 = (uint32_t)((uint64_t)quads * (j + 1) / cnt);
+        /* A quad is four elements of the output; P lanes share one, each adds up to eight parts at a time.  Two quads of a
+         * lane are loaded together, and all loads are issued before the first is used: a part is one access to L2, and
+         * one after the other they took 10 to 15 us of a call. */
         uint32_t P = 1;
-        while (P < cnt && P < 32u) P <<= 1;
-        const uint32_t p = lane & (P - 1u), at_once = 32u / P * CONSUMERS;
-        for (uint32_t base = g0; base < g1; base += at_once) {
-            const uint32_t gi = base + w * (32u / P) + lane / P;
-            const bool act = gi < g1;
-            const uint32_t r = act ? gi / (D / 4) : 0, d = act ? (gi - r * (D / 4)) * 4 : 0;
-            float M = -INFINITY;
-            for (uint32_t s = p; s < cnt; s += P) M = fmaxf(M, ld_cg_f(part(i0 + s, s == 0 ? 1 : 0) + KV_ROWS * D + r));
-            for (uint32_t o = P >> 1; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-            const float c = M == -INFINITY ? 0.f : M;
-            float l = 0.f, x[4] = { 0.f, 0.f, 0.f, 0.f };
-            for (uint32_t s = p; s < cnt; s += P) {
-                const float* q_ = part(i0 + s, s == 0 ? 1 : 0);
-                const float a = exp2_fast(ld_cg_f(q_ + KV_ROWS * D + r) - c);
-                l += a * ld_cg_f(q_ + KV_ROWS * (D + 1) + r);
-                const uint4 y = ld_cg_v4(q_ + r * D + d);
-                x[0] += a * __uint_as_float(y.x); x[1] += a * __uint_as_float(y.y); x[2] += a * __uint_as_float(y.z); x[3] += a * __uint_as_float(y.w);
-            }
-            for (uint32_t o = P >> 1; o > 0; o >>= 1) {
-                l += __shfl_xor_sync(0xffffffffu, l, o);
+        while (P * 8 < cnt && P < 32u) P <<= 1;
+        const uint32_t p = lane & (P - 1u), at_once = 32u / P;
+        for (uint32_t base = g0; base < g1; base += 2 * at_once) {
+            float M[2], l[2], x[2][4];
+            uint32_t r[2], d[2];
+            bool act[2];
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
+            for (int e = 0; e < 2; e++) {
+                const uint32_t gi = base + e * at_once + lane / P;
+                act[e] = gi < g1;
+                r[e] = act[e] ? gi / (D / 4) : 0;
+                d[e] = act[e] ? (gi - r[e] * (D / 4)) * 4 : 0;
+                M[e] = -INFINITY; l[e] = 0.f;
+                x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.f;
             }
-            if (act && p == 0) {
-                const uint32_t hq = h * group + r0 + r;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                uint16_t* dst = out + b * o_sb + hq * o_sh + d;
-                store_pair(dst, x[0] * inv, x[1] * inv);
-                store_pair(dst + 2, x[2] * inv, x[3] * inv);
-                if (lse && d == 0) lse[(size_t)b * n_q_heads + hq] = lse_of(M, l);
+            for (uint32_t s0 = 0; s0 < cnt; s0 += 8 * P) {
+                float2 ml[2][8];
+                uint4 y[2][8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t s = s0 + k * P + p;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        ml[e][k] = make_float2(-INFINITY, 0.f);
+                        y[e][k] = make_uint4(0, 0, 0, 0);
+                        if (s < cnt && act[e]) {
+                            const float* y_ = part(i0 + s, s == 0 ? 1 : 0);
+                            ml[e][k] = ld_cg_f2(y_ + KV_ROWS * D + 2 * r[e]);
+                            y[e][k] = ld_cg_v4(y_ + r[e] * D + d[e]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float m = M[e];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) m = fmaxf(m, ml[e][k].x);
+                    const float c = m == -INFINITY ? 0.f : m, a = exp2_fast(M[e] - c);
+                    M[e] = m;
+                    l[e] *= a;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[e][i] *= a;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float a1 = exp2_fast(ml[e][k].x - c);
+                        l[e] += ml[e][k].y * a1;
+                        x[e][0] += __uint_as_float(y[e][k].x) * a1; x[e][1] += __uint_as_float(y[e][k].y) * a1;
+                        x[e][2] += __uint_as_float(y[e][k].z) * a1; x[e][3] += __uint_as_float(y[e][k].w) * a1;
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float all = M[e];
+                for (uint32_t o = P >> 1; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+                const float a = exp2_fast(M[e] - (all == -INFINITY ? 0.f : all));
+                l[e] *= a;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[e][i] *= a;
+                for (uint32_t o = P >> 1; o > 0; o >>= 1) {
+                    l[e] += __shfl_xor_sync(0xffffffffu, l[e], o);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[e][i] += __shfl_xor_sync(0xffffffffu, x[e][i], o);
+                }
+                if (act[e] && p == 0) {
+                    const uint32_t hq = h * group + r0 + r[e];
+                    const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
+                    uint16_t* dst = out + b * o_sb + hq * o_sh + d[e];
+                    store_pair(dst, x[e][0] * inv, x[e][1] * inv);
+                    store_pair(dst + 2, x[e][2] * inv, x[e][3] * inv);
+                    if (lse && d[e] == 0) lse[(size_t)b * n_q_heads + hq] = lse_of(all, l[e]);
+                }
             }
         }
     }
@@ -656,13 +737,11 @@ struct KvAttendWork {
     {
         /* stages on 1 KB boundaries: the addresses within one are formed with XOR */
         uint8_t* const mem = bam_dyn_smem + (0u - smem_u32(bam_dyn_smem)) % 1024u;
-        shared_t& sh = *reinterpret_cast<shared_t*>(mem + ring_bytes);
+        kv_shared_t& sh = *reinterpret_cast<kv_shared_t*>(mem + ring_bytes);
         const uint32_t ring = smem_u32(mem), t = threadIdx.x, lane = t & 31u, w = t >> 5;
-        const uint32_t units = L.n_kv_heads * tiles, S = stages();
-        if (t < S) {
-            mbar_init(smem_u32(&sh.full[t]), 1);
-        }
-        if (t < KV_AHEAD) sh.tag[t] = 0;
+        const uint32_t units = L.n_kv_heads * tiles;
+        if (t < KV_WORKERS * KV_STAGES_MAX) mbar_init(smem_u32(&sh.full[0][t]), 1);
+        if (t < KV_WORKERS * KV_AHEAD) sh.tag[0][t] = 0;
         if (t == 0) sh.abort = status_bad(L.r.cache.status) ? 1u : 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -670,35 +749,36 @@ struct KvAttendWork {
         const uint32_t run = (batch + threads - 1) / threads;
         const uint32_t s0 = t * run < batch ? t * run : batch, s1 = s0 + run < batch ? s0 + run : batch;
         uint64_t own = 0;
-        for (uint32_t b = s0; b < s1; b++) own += seen(b, vb == 0).n;
+        uint32_t longest = 0;
+        for (uint32_t b = s0; b < s1; b++) {
+            const uint32_t n = seen(b, vb == 0).n;
+            own += n;
+            longest = n > longest ? n : longest;
+        }
         uint64_t before = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t x = __shfl_up_sync(0xffffffffu, before, o);
             if (lane >= (uint32_t)o) before += x;
         }
-        if (lane == 31) sh.warp_sum[w] = before;
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        if (lane == 31) { sh.warp_sum[w] = before; sh.warp_max[w] = longest; }
         before -= own;
         __syncthreads();
         if (sh.abort) return;
         uint64_t total = 0;
 #pragma unroll
-        for (uint32_t k = 0; k < CONSUMERS + 1; k++) {
+        for (uint32_t k = 0; k < KV_WORKERS + 1; k++) {
             if (k < w) before += sh.warp_sum[k];
             total += sh.warp_sum[k];
+            longest = sh.warp_max[k] > longest ? sh.warp_max[k] : longest;
         }
         total *= units;
-        uint64_t per = (total + nvb - 1) / nvb;
-        if (per < KV_MIN_CHUNKS) per = KV_MIN_CHUNKS;
-        const uint64_t f0 = (uint64_t)vb * per, f1 = f0 + per < total ? f0 + per : total;
-        if (own && f0 >= before * units && f0 < (before + own) * units) {
-            uint64_t at = before * units;
-            for (uint32_t b = s0; b < s1; b++) {
-                const uint64_t span = (uint64_t)seen(b).n * units;
-                if (f0 < at + span) { sh.start_b = b; sh.start_pos = f0 - at; break; }
-                at += span;
-            }
-        }
+        sh.before[t] = before * units;
+        const uint64_t n_workers = (uint64_t)nvb * KV_WORKERS;
+        uint64_t per = (total + n_workers - 1) / n_workers;
+        const uint32_t least = longest < KV_MIN_CHUNKS ? longest : KV_MIN_CHUNKS;
+        if (per < least) per = least;
         /* sequences with nothing visible */
         for (uint32_t b = vb; b < batch; b += nvb) {
             if (seen(b).n == 0) {
@@ -710,13 +790,21 @@ struct KvAttendWork {
             }
         }
         __syncthreads();
-        if (f0 < f1) {
-            if (w == CONSUMERS) pin_ahead(sh, f0, f1, vb);
-            else consume(sh, ring, f0, f1, per, vb);
+        /* neighbours in the list on different SMs: the workers of a short list spread out */
+        const uint32_t worker = w * nvb + vb;
+        if (w < KV_WORKERS) {
+            const kv_place_t from = cut(sh, worker, per, total), to = cut(sh, worker + 1ull, per, total);
+            if (lane == 0) { sh.from[w] = from; sh.chunks[w] = (uint32_t)(to.f - from.f); }
         }
         __syncthreads();
-        /* given up: pages that were pinned and never copied */
-        if (sh.abort && t < KV_AHEAD && (sh.tag[t] & 1u) && sh.pinned[t].slot != BAM_SLOT_NONE) L.r.release_page(sh.pinned[t].slot, 1);
+        if (w < KV_WORKERS) {
+            if (sh.chunks[w]) work(sh, ring, per, worker);
+        } else pin_ahead(sh, vb);
+        __syncthreads();
+        if (sh.abort && t < KV_WORKERS * KV_AHEAD && (sh.tag[0][t] & 1u)) {            /* given up: what was pinned and never copied */
+            const kv_pinned_t& e = sh.pinned[0][t];
+            for (uint32_t k = 0; k < CS / piece; k++) if (e.slot[k] != BAM_SLOT_NONE) L.r.release_page(e.slot[k], 1);
+        }
     }
 };
 
@@ -740,28 +828,33 @@ static int launch_attend_as(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     uint8_t* base = (uint8_t*)scratch;
     const uint32_t most = kv_most_blocks(a);
     w.arrived = (uint32_t*)(base + sizeof(kv_launch_words_t));
-    w.parts = (float*)(base + kv_parts_at(most));
+    w.parts = (float*)(base + kv_parts_at(most * KV_WORKERS));
+    w.piece = L.block_tokens % CS == 0 ? CS : 16;
+    /* what all workers may hold pinned is at most half of the cache (one chunk each where that is too little) */
+    const uint64_t share = a->pc->d.n_slots / 2 / ((uint64_t)most * KV_WORKERS * (CS / w.piece));
+    w.ahead = share < 1 ? 1u : share < KV_AHEAD ? (uint32_t)share : KV_AHEAD;
     /* no more blocks than the longest sequences could keep busy */
-    uint64_t chunks = (uint64_t)p->table_width * (L.block_tokens / CS);
+    uint64_t chunks = ((uint64_t)p->table_width * L.block_tokens + CS - 1) / CS;
     if (p->window > 0) {
         const uint64_t seen = (uint64_t)p->window / CS + (uint64_t)(p->sinks < (1ll << 40) ? p->sinks : (1ll << 40)) / CS + 4;
         if (seen < chunks) chunks = seen;
     }
-    const uint64_t want = (chunks * p->batch * L.n_kv_heads * w.tiles + KV_MIN_CHUNKS - 1) / KV_MIN_CHUNKS;
-    return kv_launch(a->pc->ctrl, w, want < most ? want : most, scratch, sizeof(kv_launch_words_t) + 4 * (size_t)most, (cudaStream_t)stream);
+    const uint32_t least = chunks < KV_MIN_CHUNKS ? (uint32_t)chunks : KV_MIN_CHUNKS;
+    const uint64_t workers = (chunks * p->batch * L.n_kv_heads * w.tiles + least - 1) / least;
+    const uint64_t want = (workers + KV_WORKERS - 1) / KV_WORKERS;
+    return kv_launch(a->pc->ctrl, w, want < most ? want : most, scratch, sizeof(kv_launch_words_t) + 4 * (size_t)most * KV_WORKERS, (cudaStream_t)stream);
 }
 
 template <class T>
 int kv_launch_attend(bam_array* a, const kv_layout_d_t& L, const bam_kv_attend_t* p, void* scratch, void* stream)
 {
-    /* chunks of 32 tokens halve what a chunk costs beside its products (softmax statistics, barriers); blocks that they
-     * do not divide, and wide heads, whose registers are taken, go in chunks of 16 */
-    const bool by32 = L.block_tokens % 32 == 0;
+    /* chunks of 32 tokens halve what a chunk costs beside its products (softmax statistics, barriers); above 128
+     * dimensions their sums and scores do not fit the registers */
     switch (L.head_dim) {
-    case 64: return by32 ? launch_attend_as<T, 64, 32, true>(a, L, p, scratch, stream) : launch_attend_as<T, 64, 16, true>(a, L, p, scratch, stream);
-    case 80: return launch_attend_as<T, 80, 16, true>(a, L, p, scratch, stream);
-    case 96: return launch_attend_as<T, 96, 16, true>(a, L, p, scratch, stream);
-    case 128: return by32 ? launch_attend_as<T, 128, 32, true>(a, L, p, scratch, stream) : launch_attend_as<T, 128, 16, true>(a, L, p, scratch, stream);
+    case 64: return launch_attend_as<T, 64, 32, true>(a, L, p, scratch, stream);
+    case 80: return launch_attend_as<T, 80, 32, true>(a, L, p, scratch, stream);
+    case 96: return launch_attend_as<T, 96, 32, true>(a, L, p, scratch, stream);
+    case 128: return launch_attend_as<T, 128, 32, true>(a, L, p, scratch, stream);
     case 256: return launch_attend_as<T, 256, 16, true>(a, L, p, scratch, stream);
     default: break;
     }

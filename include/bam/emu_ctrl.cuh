@@ -393,6 +393,11 @@ BAM_DEV void emu_controller_main(const bam_emu_d_t& c, uint8_t* smem)
 #ifdef BAM_PROFILE
         long long pt = clock64();
 #endif
+        /* the words that end the launch are asked for beside the doorbells, not after them: an idle processor sees the
+         * end of its launch one round trip later instead of three */
+        uint32_t end_word = 0;
+        if (lane == 1) end_word = c.sys_scope ? ld_relaxed_sys(c.consumers_remaining) : ld_relaxed_gpu(c.consumers_remaining);
+        else if (lane == 2) end_word = ld_relaxed_gpu(&c.status->code);
         if (lane == 0 && !spare) {
             for (uint32_t r = 0; r < rounds && n == 0; r++) {
                 n = emu_reserve(c, q, want, fetch, cqbase);
@@ -478,9 +483,10 @@ BAM_DEV void emu_controller_main(const bam_emu_d_t& c, uint8_t* smem)
             idle_ns = 32; idle_rounds = 0;
             continue;
         }
+        const uint32_t remaining = __shfl_sync(full, end_word, 1), code = __shfl_sync(full, end_word, 2);
         uint32_t stop = 0;
         if (lane == 0) {
-            stop = ((c.sys_scope ? ld_acquire_sys(c.consumers_remaining) : ld_acquire_gpu(c.consumers_remaining)) == 0u) || status_bad(c.status);
+            stop = remaining == 0u || code != 0u;
             if (!stop && ((++idle_rounds) & 63u) == 0u && global_timer_ns() - t_start > c.status->launch_timeout_ns) {
                 status_fail(c.status, BAM_ETIMEDOUT, BAM_AT_LAUNCH, 0);
                 stop = 1;
