@@ -962,7 +962,7 @@ static int cache_reset_device(bam_cache* pc)
 {
     k_init_cache<<<pc->ctrl->num_sms * 4, 256>>>(pc->d.slots, pc->d.n_slots, pc->d.table, pc->n_buckets * BAM_BUCKET_WORDS);
     CK(cudaGetLastError());
-    CK(cudaMemset(pc->d.clock_hand, 0, 8 * BAM_HAND_STRIDE * BAM_MAX_HANDS));
+    CK(cudaMemset(pc->d.clock_hand, 0, 8 * BAM_HAND_STRIDE * (BAM_MAX_HANDS + 1)));
     CK(cudaMemset(pc->d.stats, 0, sizeof(bam_stat_stripe_t) * BAM_STAT_STRIPES));
     CK(cudaDeviceSynchronize());
     return BAM_OK;
@@ -1036,7 +1036,7 @@ extern "C" int bam_cache_create_multi(bam_cache_t* out, const bam_ctrl_t* ctrls,
     d.base_addr = reinterpret_cast<uint8_t*>(((uintptr_t)pc->base_raw + 4095) / 4096 * 4096);
     alloc((void**)&d.slots, n_pages * sizeof(bam_slot_t));
     alloc((void**)&d.table, pc->n_buckets * BAM_BUCKET_WORDS * 4);
-    alloc((void**)&d.clock_hand, 8 * BAM_HAND_STRIDE * BAM_MAX_HANDS);
+    alloc((void**)&d.clock_hand, 8 * BAM_HAND_STRIDE * (BAM_MAX_HANDS + 1));
     alloc((void**)&d.stats, sizeof(bam_stat_stripe_t) * BAM_STAT_STRIPES);
     alloc((void**)&d.range_page_starts, 8 * BAM_MAX_RANGES);
     alloc((void**)&d.range_dists, 4 * BAM_MAX_RANGES);
@@ -1135,7 +1135,7 @@ extern "C" int bam_cache_invalidate_async(bam_cache_t pc, void* stream)
     cudaStream_t s = (cudaStream_t)stream;
     k_init_cache<<<pc->ctrl->num_sms * 4, 256, 0, s>>>(pc->d.slots, pc->d.n_slots, pc->d.table, pc->n_buckets * BAM_BUCKET_WORDS);
     CK(cudaGetLastError());
-    CK(cudaMemsetAsync(pc->d.clock_hand, 0, 8 * BAM_HAND_STRIDE * BAM_MAX_HANDS, s));
+    CK(cudaMemsetAsync(pc->d.clock_hand, 0, 8 * BAM_HAND_STRIDE * (BAM_MAX_HANDS + 1), s));
     return BAM_OK;
 }
 

@@ -318,7 +318,8 @@ typedef struct {
     uint32_t bucket_mask;        /* n_buckets - 1 (power of two)                 */
     uint32_t n_blocks_per_page;  /* logical blocks per cache page                */
     uint64_t* clock_hand;        /* the sweep positions (page_ticket in the reference): n_hands counters, one per
-                                  * 32-byte sector; hand h sweeps the slots s with s % n_hands == h */
+                                  * 32-byte sector; hand h sweeps the slots s with s % n_hands == h; behind them, at
+                                  * BAM_MAX_HANDS, the number of slots that have been given out for the first time */
     Controller* d_ctrl;          /* backing controller (the first one when there are several) */
     Controller** d_ctrls;        /* [n_ctrls] all backing controllers             */
     uint32_t n_ctrls;

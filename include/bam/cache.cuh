@@ -16,7 +16,7 @@
  *    validate the slot's tag; eviction claims a slot with a 32-bit CAS that only succeeds on
  *    an unpinned, non-busy word, so a pinned page can never be recycled and a reader that
  *    raced with a recycle sees a tag mismatch, undoes its pin and looks the page up again.
- *  - Eviction is a clock sweep over the slots (the reference's page_ticket hand, :1802), with up to 16 hands
+ *  - Slots that were never used go out first; then eviction is a clock sweep over the slots (the reference's page_ticket hand, :1802), with up to 16 hands
  *    for a large cache: the SMs are dealt over the hands and every hand sweeps its own residue class of
  *    slots, so the misses of the whole GPU do not meet on one counter.
  *  - Read-only element accesses to resident pages take no pin at all: they validate a recycle
@@ -137,6 +137,13 @@ BAM_DEV uint32_t find_slot(const page_cache_d_t& pc, uint32_t max_tries = 0xffff
 {
     spin_t sp;
     if (dirty_tag) *dirty_tag = BAM_TAG_NONE;
+    /* Slots that were never used go out first, in order.  The hands alone would evict while there are some left: the
+     * hand of SMs that miss more than others comes round before the others have got that far. */
+    uint64_t* unused = pc.clock_hand + (size_t)BAM_MAX_HANDS * BAM_HAND_STRIDE;
+    if (ld_relaxed_gpu(unused) < pc.n_slots) {
+        const uint64_t t = atom_add_relaxed(unused, 1ull);
+        if (t < pc.n_slots && atom_cas_acquire(&pc.slots[t].state, 0u, BAM_BUSY) == 0u) { BAM_PROF_ADD(pc.status, 12, 1); return (uint32_t)t; }
+    }
 #pragma unroll 1
     for (uint32_t tries = 1;; tries++) {
         if (tries > max_tries) return BAM_SLOT_NONE;          /* caller asked for a bounded attempt */
