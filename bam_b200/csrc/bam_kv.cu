@@ -27,63 +27,101 @@ struct kv_rope_d_t {
     int64_t stride;
     uint32_t rotary_dim;         /* 0: no rotation                                             */
     uint32_t style;              /* BAM_KV_ROPE_HALF / BAM_KV_ROPE_PAIRS                       */
+    uint32_t vec;                /* rows of cos and sin lie on 16-byte boundaries               */
 };
 
-/* One row of a head: G lanes (a power of two, at least head_dim / 8) hold eight elements each.  All lanes of the
- * warp call it.  y = x * rsqrt(mean(x^2) + eps) * w, then the rotation; everything in 32 bits, rounded once. */
-template <class T>
-BAM_DEV uint4 kv_transform(uint4 raw, uint32_t c, uint32_t G, uint32_t head_dim, const uint16_t* norm, float eps,
-                           const kv_rope_d_t& rope, int64_t pos)
+/* A lane holds two 16-byte chunks of a row: the two halves of eight rotated pairs where there are such (chunks j and
+ * j + rotary_dim / 16, or 2 j and 2 j + 1 for neighbouring pairs), so that a rotation needs no other lane and one set of
+ * eight cosines and sines serves sixteen elements; they are loaded once per token and serve all its heads. */
+struct kv_lane_t {
+    uint32_t ca, cb;             /* the lane's chunks; ca = 0xffffffff: none                    */
+    bool turned;                 /* they hold rotated pairs                                     */
+    float c[8], s[8];            /* of the token at hand                                        */
+    uint4 wa, wb;                /* the norm's weights, of the item at hand                     */
+};
+
+BAM_DEV kv_lane_t kv_lane(uint32_t j, uint32_t chunks, const kv_rope_d_t& rope)
 {
-    if (!norm && rope.rotary_dim == 0) return raw;
-    float x[8];
-    {
-        const uint32_t w[4] = { raw.x, raw.y, raw.z, raw.w };
+    kv_lane_t n;
+    const uint32_t half = rope.rotary_dim / 16;                        /* chunks of half the rotated elements */
+    n.turned = j < half;
+    if (n.turned && rope.style == BAM_KV_ROPE_HALF) { n.ca = j; n.cb = j + half; }
+    else { n.ca = 2 * j; n.cb = 2 * j + 1; }                           /* rotary_dim and head_dim are multiples of 16 */
+    if (n.cb >= chunks) n.ca = 0xffffffffu;
 #pragma unroll
-        for (int i = 0; i < 4; i++) { const float2 f = kv_type<T>::unpack(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+    for (int i = 0; i < 8; i++) { n.c[i] = 1.f; n.s[i] = 0.f; }
+    return n;
+}
+BAM_DEV void kv_load_angle(kv_lane_t& n, uint32_t j, const kv_rope_d_t& rope, int64_t pos)
+{
+    if (!n.turned || n.ca == 0xffffffffu) return;
+    const float* c = rope.cos + pos * rope.stride + j * 8;
+    const float* s = rope.sin + pos * rope.stride + j * 8;
+    if (rope.vec) {
+        const float4 c0 = __ldg(reinterpret_cast<const float4*>(c)), c1 = __ldg(reinterpret_cast<const float4*>(c) + 1);
+        const float4 s0 = __ldg(reinterpret_cast<const float4*>(s)), s1 = __ldg(reinterpret_cast<const float4*>(s) + 1);
+        n.c[0] = c0.x; n.c[1] = c0.y; n.c[2] = c0.z; n.c[3] = c0.w; n.c[4] = c1.x; n.c[5] = c1.y; n.c[6] = c1.z; n.c[7] = c1.w;
+        n.s[0] = s0.x; n.s[1] = s0.y; n.s[2] = s0.z; n.s[3] = s0.w; n.s[4] = s1.x; n.s[5] = s1.y; n.s[6] = s1.z; n.s[7] = s1.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) { n.c[i] = __ldg(c + i); n.s[i] = __ldg(s + i); }
     }
-    const bool in_row = c * 8 < head_dim;
+}
+
+/* y = x * rsqrt(mean(x^2) + eps) * w of the row that G lanes hold, then the rotation: in 32 bits, rounded once.  All
+ * lanes of the warp call it. */
+template <class T>
+BAM_DEV void kv_transform(uint4& a, uint4& b, const kv_lane_t& n, uint32_t G, uint32_t head_dim, bool norm, float eps,
+                          const kv_rope_d_t& rope)
+{
+    if (!norm && rope.rotary_dim == 0) return;
+    float x[8], y[8];
+    {
+        const uint32_t u[4] = { a.x, a.y, a.z, a.w }, v[4] = { b.x, b.y, b.z, b.w };
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = kv_type<T>::unpack(u[i]), g = kv_type<T>::unpack(v[i]);
+            x[2 * i] = f.x; x[2 * i + 1] = f.y; y[2 * i] = g.x; y[2 * i + 1] = g.y;
+        }
+    }
     if (norm) {
         float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-        if (!in_row) ss = 0.f;
+        for (int i = 0; i < 8; i++) ss += x[i] * x[i] + y[i] * y[i];
         for (uint32_t o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float inv = rsqrtf(ss / (float)head_dim + eps);
-        if (in_row) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = x[i] * inv * kv_type<T>::to_f(norm[c * 8 + i]);
-        }
-    }
-    const uint32_t half = rope.rotary_dim >> 1;
-    if (rope.rotary_dim) {
-        if (rope.style == BAM_KV_ROPE_HALF) {
-            /* the other element of a pair lies rotary_dim / 2 away: half / 8 lanes (rotary_dim is a multiple of 16) */
-            const bool low = c * 8 < half, turned = c * 8 < rope.rotary_dim;
-            const uint32_t other = turned ? (low ? c + half / 8 : c - half / 8) : c;
-            const uint32_t src = ((threadIdx.x & 31u) & ~(G - 1u)) + other;
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = __shfl_sync(0xffffffffu, x[i], src);
-            if (turned) {
-                const uint32_t e = low ? c * 8 : c * 8 - half;
-                const float* cs = rope.cos + pos * rope.stride + e;
-                const float* sn = rope.sin + pos * rope.stride + e;
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = low ? x[i] * __ldg(cs + i) - p[i] * __ldg(sn + i) : x[i] * __ldg(cs + i) + p[i] * __ldg(sn + i);
-            }
-        } else if (c * 8 < rope.rotary_dim) {
-            const float* cs = rope.cos + pos * rope.stride + c * 4;
-            const float* sn = rope.sin + pos * rope.stride + c * 4;
+        if (n.ca != 0xffffffffu) {
+            const uint32_t w[8] = { n.wa.x, n.wa.y, n.wa.z, n.wa.w, n.wb.x, n.wb.y, n.wb.z, n.wb.w };
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float a = x[2 * i], b = x[2 * i + 1], cc = __ldg(cs + i), ss = __ldg(sn + i);
-                x[2 * i] = a * cc - b * ss;
-                x[2 * i + 1] = b * cc + a * ss;
+                const float2 f = kv_type<T>::unpack(w[i]), g = kv_type<T>::unpack(w[4 + i]);
+                x[2 * i] = x[2 * i] * inv * f.x; x[2 * i + 1] = x[2 * i + 1] * inv * f.y;
+                y[2 * i] = y[2 * i] * inv * g.x; y[2 * i + 1] = y[2 * i + 1] * inv * g.y;
             }
         }
     }
-    return make_uint4(kv_type<T>::pack(x[0], x[1]), kv_type<T>::pack(x[2], x[3]), kv_type<T>::pack(x[4], x[5]), kv_type<T>::pack(x[6], x[7]));
+    if (n.turned) {
+        if (rope.style == BAM_KV_ROPE_HALF) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float p = x[i], q = y[i];
+                x[i] = p * n.c[i] - q * n.s[i];
+                y[i] = q * n.c[i] + p * n.s[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float p = x[2 * i], q = x[2 * i + 1];
+                x[2 * i] = p * n.c[i] - q * n.s[i];
+                x[2 * i + 1] = q * n.c[i] + p * n.s[i];
+                p = y[2 * i]; q = y[2 * i + 1];
+                y[2 * i] = p * n.c[4 + i] - q * n.s[4 + i];
+                y[2 * i + 1] = q * n.c[4 + i] + p * n.s[4 + i];
+            }
+        }
+    }
+    a = make_uint4(kv_type<T>::pack(x[0], x[1]), kv_type<T>::pack(x[2], x[3]), kv_type<T>::pack(x[4], x[5]), kv_type<T>::pack(x[6], x[7]));
+    b = make_uint4(kv_type<T>::pack(y[0], y[1]), kv_type<T>::pack(y[2], y[3]), kv_type<T>::pack(y[4], y[5]), kv_type<T>::pack(y[6], y[7]));
 }
 
 /* Pins the pages of up to 32 rows, one per lane, and hands the rows of every page that could be pinned to `rows`,
@@ -113,6 +151,15 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
     return true;
 }
 
+/* The work is cut into items of tokens_per_item consecutive tokens: KV_Q_HEADS of their query heads, or the keys and values
+ * of the runs that begin there.  A run is the tokens in a row that go to one block: one warp writes it, to the end of the
+ * run and not of the item, and pins each head's page once.  (Warps that miss the same page at once claim a slot each: a
+ * prompt whose pages were written by two warps each evicted half of a cache that had room for all of it.)  Bytes bound it (every row is read and
+ * written once); what it needs for that is rows in flight: KV_ROWS_AHEAD rows of a lane are loaded before the first is
+ * worked on, and angles are loaded once per token and item. */
+#define KV_Q_HEADS 16u
+#define KV_ROWS_AHEAD 4
+
 template <class T>
 struct KvAppendWork {
     static constexpr int threads = BAM_THREADS, min_blocks = 2;
@@ -122,8 +169,8 @@ struct KvAppendWork {
     uint16_t* q_out;
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh;      /* element strides of token and head */
     uint64_t n_tokens;
-    uint32_t n_q_heads, lanes_per_row, tokens_per_item;
-    uint32_t vec;                                                  /* bit 0: q, 1: k, 2: v, 3: q_out lie on 16-byte boundaries */
+    uint32_t n_q_heads, lanes_per_row, tokens_per_item, q_parts;
+    uint32_t vec;                                                  /* bit 0: q, 1: k, 2: v, 3: q_out, 4: q_norm, 5: k_norm lie on 16-byte boundaries */
     const int64_t* slots;
     kv_rope_d_t rope;
     const uint16_t *q_norm, *k_norm;
@@ -140,71 +187,138 @@ struct KvAppendWork {
         return -1;
     }
 
+    /* the block a token goes to; ~0: none, it is padding or its slot is no slot */
+    BAM_DEV uint64_t block_of(uint64_t t) const
+    {
+        const int64_t slot = slots[t];
+        if (slot < 0) return ~0ull;
+        if ((uint64_t)slot >= L.n_blocks * L.block_tokens) { L.bad_index((uint64_t)slot); return ~0ull; }
+        return (uint64_t)slot / L.block_tokens;
+    }
+
+    /* rows [0, n) of one token, head by head: heads h0 + r */
+    BAM_DEV void queries(uint64_t t, uint32_t h0, uint32_t n, const kv_lane_t& ln, uint32_t G, uint32_t grp) const
+    {
+        const uint32_t rows = 32u / G;
+        const uint16_t* src = q + (int64_t)t * q_st;
+        uint16_t* dst = q_out + (int64_t)t * qo_st;
+        for (uint32_t r0 = 0; r0 < n; r0 += rows * KV_ROWS_AHEAD) {
+            uint4 a[KV_ROWS_AHEAD], b[KV_ROWS_AHEAD];
+#pragma unroll
+            for (int i = 0; i < KV_ROWS_AHEAD; i++) {
+                const uint32_t r = r0 + i * rows + grp;
+                a[i] = b[i] = make_uint4(0, 0, 0, 0);
+                if (r < n && ln.ca != 0xffffffffu) {
+                    a[i] = kv_load8(src + (h0 + r) * q_sh + ln.ca * 8, vec & 1u);
+                    b[i] = kv_load8(src + (h0 + r) * q_sh + ln.cb * 8, vec & 1u);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < KV_ROWS_AHEAD; i++) {
+                if (r0 + i * rows >= n) break;
+                const uint32_t r = r0 + i * rows + grp;
+                kv_transform<T>(a[i], b[i], ln, G, L.head_dim, q_norm != nullptr, eps, rope);
+                if (r < n && ln.ca != 0xffffffffu) {
+                    kv_store8(dst + (h0 + r) * qo_sh + ln.ca * 8, a[i], vec & 8u);
+                    kv_store8(dst + (h0 + r) * qo_sh + ln.cb * 8, b[i], vec & 8u);
+                }
+            }
+        }
+    }
+
+    /* keys and values of one token into row `row` of the pages at `addr` (lane: head h0 + lane, those of mask m) */
+    BAM_DEV void keys(uint64_t t, uint32_t row, uint32_t h0, uint32_t n, uint32_t m, uint64_t addr, const kv_lane_t& ln, uint32_t G, uint32_t grp) const
+    {
+        const uint32_t rows = 32u / G;
+        const uint16_t *ks = k + (int64_t)t * k_st, *vs = v + (int64_t)t * v_st;
+        const uint32_t oa = row * L.row_bytes() + L.swizzle(row, ln.ca) * 16u, ob = row * L.row_bytes() + L.swizzle(row, ln.cb) * 16u;
+        for (uint32_t r0 = 0; r0 < n; r0 += rows * 2) {
+            uint4 ka[2], kb[2], va[2], vb[2];
+            uint64_t page[2];
+            bool act[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t r = r0 + i * rows + grp;
+                page[i] = __shfl_sync(0xffffffffu, addr, r & 31u);
+                act[i] = r < n && ((m >> (r & 31u)) & 1u) && ln.ca != 0xffffffffu;
+                ka[i] = kb[i] = va[i] = vb[i] = make_uint4(0, 0, 0, 0);
+                if (act[i]) {
+                    ka[i] = kv_load8(ks + (h0 + r) * k_sh + ln.ca * 8, vec & 2u);
+                    kb[i] = kv_load8(ks + (h0 + r) * k_sh + ln.cb * 8, vec & 2u);
+                    va[i] = kv_load8(vs + (h0 + r) * v_sh + ln.ca * 8, vec & 4u);
+                    vb[i] = kv_load8(vs + (h0 + r) * v_sh + ln.cb * 8, vec & 4u);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                kv_transform<T>(ka[i], kb[i], ln, G, L.head_dim, k_norm != nullptr, eps, rope);
+                if (act[i]) {
+                    uint8_t* p = reinterpret_cast<uint8_t*>(page[i]);
+                    *reinterpret_cast<uint4*>(p + oa) = ka[i];
+                    *reinterpret_cast<uint4*>(p + ob) = kb[i];
+                    *reinterpret_cast<uint4*>(p + L.v_offset() + oa) = va[i];
+                    *reinterpret_cast<uint4*>(p + L.v_offset() + ob) = vb[i];
+                }
+            }
+        }
+    }
+
     __device__ void operator()(uint32_t vb, uint32_t nvb) const
     {
-        const uint32_t lane = threadIdx.x & 31u;
-        const uint64_t warp = ((uint64_t)vb * blockDim.x + threadIdx.x) >> 5, nwarps = ((uint64_t)nvb * blockDim.x) >> 5;
-        const uint32_t G = lanes_per_row, rows = 32u / G, c = lane & (G - 1u), grp = lane / G;
-        const bool in_row = c < L.chunks;
+        const uint32_t full = 0xffffffffu, lane = threadIdx.x & 31u;
+        const uint64_t warp = (uint64_t)(threadIdx.x >> 5) * nvb + vb, nwarps = (uint64_t)nvb * (blockDim.x >> 5);
+        const uint32_t G = lanes_per_row, j = lane & (G - 1u), grp = lane / G;
         if (status_bad(L.r.cache.status)) return;
-        /* keys and values: an item is tokens_per_item tokens of one head */
+        kv_lane_t ln = kv_lane(j, L.chunks, rope);
         const uint64_t groups = (n_tokens + tokens_per_item - 1) / tokens_per_item;
-        for (uint64_t it = warp; it < groups * L.n_kv_heads; it += nwarps) {
-            const uint32_t h = (uint32_t)(it % L.n_kv_heads);
-            const uint64_t t0 = it / L.n_kv_heads * tokens_per_item;
-            const uint64_t t = t0 + lane;
-            int64_t slot = -1, pos = 0;
-            if (lane < tokens_per_item && t < n_tokens) {
-                slot = slots[t];
-                if (slot >= 0 && (uint64_t)slot >= L.n_blocks * L.block_tokens) {
-                    L.bad_index((uint64_t)slot);
-                    slot = -1;
-                }
-                if (slot >= 0) pos = position(t, false);
-                if (pos < 0) slot = -1;
+        for (uint64_t it = warp; it < groups * (1 + q_parts); it += nwarps) {
+            const uint32_t part = (uint32_t)(it % (1 + q_parts));
+            const uint64_t t0 = it / (1 + q_parts) * tokens_per_item;
+            const uint32_t nt = n_tokens - t0 < tokens_per_item ? (uint32_t)(n_tokens - t0) : tokens_per_item;
+            const uint16_t* norm = part ? q_norm : k_norm;
+            if (norm && ln.ca != 0xffffffffu) {
+                ln.wa = kv_load8(norm + ln.ca * 8, vec & (part ? 16u : 32u));
+                ln.wb = kv_load8(norm + ln.cb * 8, vec & (part ? 16u : 32u));
             }
-            const uint32_t row = slot >= 0 ? (uint32_t)((uint64_t)slot % L.block_tokens) : 0;
-            const uint64_t page = slot >= 0 ? L.page_of((uint64_t)slot / L.block_tokens, h) : 0;
-            const bool ok = kv_with_pages(L, slot >= 0, page, true, (uint32_t)warp, [&](uint32_t m, uint64_t addr) {
-                for (uint32_t i = 0; i < tokens_per_item; i += rows) {
-                    const uint32_t src = (i + grp) & 31u;
-                    if (!((m >> i) & ((rows == 32u) ? 0xffffffffu : (1u << rows) - 1u))) continue;
-                    const bool act = in_row && i + grp < tokens_per_item && ((m >> src) & 1u);
-                    const uint64_t base = __shfl_sync(0xffffffffu, addr, src);
-                    const uint32_t rr = __shfl_sync(0xffffffffu, row, src);
-                    const int64_t pp = __shfl_sync(0xffffffffu, pos, src);
-                    uint4 kk = make_uint4(0, 0, 0, 0), vv = kk;
-                    if (act) {
-                        kk = kv_load8(k + (int64_t)(t0 + src) * k_st + h * k_sh + c * 8, vec & 2u);
-                        vv = kv_load8(v + (int64_t)(t0 + src) * v_st + h * v_sh + c * 8, vec & 4u);
-                    }
-                    kk = kv_transform<T>(kk, c, G, L.head_dim, k_norm, eps, rope, pp);
-                    if (act) {
-                        uint8_t* p = reinterpret_cast<uint8_t*>(base) + rr * L.row_bytes() + L.swizzle(rr, c) * 16u;
-                        *reinterpret_cast<uint4*>(p) = kk;
-                        *reinterpret_cast<uint4*>(p + L.v_offset()) = vv;
-                    }
+            if (part) {
+                const uint32_t h0 = (part - 1) * KV_Q_HEADS, n = n_q_heads - h0 < KV_Q_HEADS ? n_q_heads - h0 : KV_Q_HEADS;
+                const int64_t pos = lane < nt ? position(t0 + lane, slots[t0 + lane] < 0) : 0;
+                for (uint32_t i = 0; i < nt; i++) {
+                    const int64_t p = __shfl_sync(full, pos, i);
+                    if (p < 0) continue;
+                    kv_load_angle(ln, j, rope, p);
+                    queries(t0 + i, h0, n, ln, G, grp);
                 }
-            });
-            if (!ok) return;
-        }
-        /* queries */
-        if (!q) return;
-        const uint64_t n_rows = n_tokens * n_q_heads;
-        for (uint64_t r0 = warp * rows; r0 < n_rows; r0 += nwarps * rows) {
-            const uint64_t rr = r0 + grp;
-            const bool act = in_row && rr < n_rows;
-            const uint64_t t = act ? rr / n_q_heads : 0;
-            const uint32_t h = act ? (uint32_t)(rr % n_q_heads) : 0;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            int64_t pos = 0;
-            if (act) {
-                x = kv_load8(q + (int64_t)t * q_st + h * q_sh + c * 8, vec & 1u);
-                pos = position(t, slots[t] < 0);
-                if (pos < 0) pos = 0;
+                continue;
             }
-            x = kv_transform<T>(x, c, G, L.head_dim, q_norm, eps, rope, pos);
-            if (act) kv_store8(q_out + (int64_t)t * qo_st + h * qo_sh + c * 8, x, vec & 8u);
+            const uint64_t mine = lane < nt ? block_of(t0 + lane) : ~0ull;
+            const uint64_t before = lane < nt && t0 + lane > 0 ? block_of(t0 + lane - 1) : ~0ull;
+            for (uint32_t begins = __ballot_sync(full, mine != ~0ull && mine != before); begins; begins &= begins - 1) {
+                const uint32_t first = __ffs(begins) - 1;
+                const uint64_t at = __shfl_sync(full, mine, first);
+                for (uint64_t t1 = t0 + first;; t1 += 32) {          /* 32 tokens of the run at a time */
+                    const uint64_t t = t1 + lane;
+                    const bool here = t < n_tokens && block_of(t) == at;
+                    const uint32_t gap = ~__ballot_sync(full, here);
+                    const uint32_t in_run = gap ? (1u << (__ffs(gap) - 1)) - 1u : full;
+                    const bool live = (in_run >> lane) & 1u;
+                    const int64_t pos = live ? position(t, false) : 0;
+                    const uint32_t row = live ? (uint32_t)((uint64_t)slots[t] % L.block_tokens) : 0;
+                    const uint32_t run = in_run & __ballot_sync(full, pos >= 0);
+                    for (uint32_t h0 = 0; h0 < L.n_kv_heads && run; h0 += 32) {
+                        const uint32_t n = L.n_kv_heads - h0 < 32u ? L.n_kv_heads - h0 : 32u;
+                        const bool ok = kv_with_pages(L, lane < n, L.page_of(at, h0 + lane), true, (uint32_t)warp, [&](uint32_t m, uint64_t addr) {
+                            for (uint32_t left = run; left; left &= left - 1) {
+                                const uint32_t i = __ffs(left) - 1;
+                                kv_load_angle(ln, j, rope, __shfl_sync(full, pos, i));
+                                keys(t1 + i, __shfl_sync(full, row, i), h0, n, m, addr, ln, G, grp);
+                            }
+                        });
+                        if (!ok) return;
+                    }
+                    if (gap) break;
+                }
+            }
         }
     }
 };
@@ -244,22 +358,31 @@ struct KvGatherWork {
             }
             const uint32_t row = slot >= 0 ? (uint32_t)((uint64_t)slot % L.block_tokens) : 0;
             const uint64_t page = slot >= 0 ? L.page_of((uint64_t)slot / L.block_tokens, h) : 0;
+            /* KV_ROWS_AHEAD rows of a lane are loaded before the first is stored: bytes bound this, if enough of them are
+             * under way */
             auto copy = [&](uint32_t m, uint64_t addr) {
-                for (uint32_t i = 0; i < tokens_per_item; i += rows) {
-                    const uint32_t src = (i + grp) & 31u;
-                    const bool act = in_row && i + grp < tokens_per_item && ((m >> src) & 1u);
-                    const uint64_t base = __shfl_sync(0xffffffffu, addr, src);
-                    const uint32_t rr = __shfl_sync(0xffffffffu, row, src);
-                    if (act) {
-                        uint4 kk = make_uint4(0, 0, 0, 0), vv = kk;
-                        if (base) {
+                for (uint32_t i0 = 0; i0 < tokens_per_item; i0 += rows * KV_ROWS_AHEAD) {
+                    uint4 kk[KV_ROWS_AHEAD], vv[KV_ROWS_AHEAD];
+#pragma unroll
+                    for (int e = 0; e < KV_ROWS_AHEAD; e++) {
+                        const uint32_t i = i0 + e * rows, src = (i + grp) & 31u;
+                        const uint64_t base = __shfl_sync(0xffffffffu, addr, src);
+                        const uint32_t rr = __shfl_sync(0xffffffffu, row, src);
+                        kk[e] = vv[e] = make_uint4(0, 0, 0, 0);
+                        if (in_row && i + grp < tokens_per_item && ((m >> src) & 1u) && base) {
                             /* past L1: a slot can hold another page now than earlier in this launch */
                             const uint8_t* p = reinterpret_cast<const uint8_t*>(base) + rr * L.row_bytes() + L.swizzle(rr, c) * 16u;
-                            kk = ld_cg_v4(p);
-                            vv = ld_cg_v4(p + L.v_offset());
+                            kk[e] = ld_cg_v4(p);
+                            vv[e] = ld_cg_v4(p + L.v_offset());
                         }
-                        kv_store8(k + (int64_t)(t0 + src) * k_st + h * k_sh + c * 8, kk, vec & 1u);
-                        kv_store8(v + (int64_t)(t0 + src) * v_st + h * v_sh + c * 8, vv, vec & 2u);
+                    }
+#pragma unroll
+                    for (int e = 0; e < KV_ROWS_AHEAD; e++) {
+                        const uint32_t i = i0 + e * rows, src = (i + grp) & 31u;
+                        if (in_row && i + grp < tokens_per_item && ((m >> src) & 1u)) {
+                            kv_store8(k + (int64_t)(t0 + src) * k_st + h * k_sh + c * 8, kk[e], vec & 1u);
+                            kv_store8(v + (int64_t)(t0 + src) * v_st + h * v_sh + c * 8, vv[e], vec & 2u);
+                        }
                     }
                 }
             };
@@ -303,11 +426,12 @@ uint32_t lanes_of_row(uint32_t chunks) { uint32_t g = 1; while (g < chunks) g <<
 
 bool on_16(const void* p, int64_t s0, int64_t s1) { return ((uintptr_t)p & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0; }
 
-/* tokens a warp takes at a time: as many as leave every warp of the GPU something to do */
-uint32_t tokens_of_item(uint64_t n_tokens, uint32_t heads, uint64_t warps)
+/* tokens a warp takes at a time: as many (up to `most`) as leave every warp of the GPU something to do.  Tokens of one
+ * block that go to different warps pin its page each, so they are kept together where that costs no parallelism. */
+uint32_t tokens_of_item(uint64_t n_tokens, uint32_t parts, uint64_t warps, uint32_t most)
 {
-    uint32_t t = KV_MAX_LANE_TOKENS;
-    while (t > 1 && (n_tokens + t - 1) / t * heads < warps) t >>= 1;
+    uint32_t t = most;
+    while (t > 1 && (n_tokens + t - 1) / t * parts < warps) t >>= 1;
     return t;
 }
 
@@ -337,19 +461,20 @@ static int launch_append(bam_array_t a, const kv_layout_d_t& L, const bam_kv_app
     w.q_st = p->q_stride[0]; w.q_sh = p->q_stride[1]; w.k_st = p->k_stride[0]; w.k_sh = p->k_stride[1];
     w.v_st = p->v_stride[0]; w.v_sh = p->v_stride[1]; w.qo_st = p->q_out_stride[0]; w.qo_sh = p->q_out_stride[1];
     w.n_tokens = p->n_tokens; w.n_q_heads = p->q ? p->n_q_heads : 0;
-    w.lanes_per_row = lanes_of_row(L.chunks);
+    w.lanes_per_row = lanes_of_row(L.chunks / 2);
+    w.q_parts = (w.n_q_heads + KV_Q_HEADS - 1) / KV_Q_HEADS;
     const uint64_t warps = (uint64_t)a->pc->ctrl->num_sms * w.min_blocks * (w.threads / 32);
-    w.tokens_per_item = tokens_of_item(p->n_tokens, L.n_kv_heads, warps);
+    w.tokens_per_item = tokens_of_item(p->n_tokens, 1 + w.q_parts, warps, 16);
     w.vec = (on_16(p->q, p->q_stride[0], p->q_stride[1]) ? 1u : 0u) | (on_16(p->k, p->k_stride[0], p->k_stride[1]) ? 2u : 0u) |
-            (on_16(p->v, p->v_stride[0], p->v_stride[1]) ? 4u : 0u) | (on_16(p->q_out, p->q_out_stride[0], p->q_out_stride[1]) ? 8u : 0u);
+            (on_16(p->v, p->v_stride[0], p->v_stride[1]) ? 4u : 0u) | (on_16(p->q_out, p->q_out_stride[0], p->q_out_stride[1]) ? 8u : 0u) |
+            (on_16(p->q_norm, 0, 0) ? 16u : 0u) | (on_16(p->k_norm, 0, 0) ? 32u : 0u);
     w.slots = p->slots;
     w.rope.positions = p->positions; w.rope.cos = p->cos; w.rope.sin = p->sin; w.rope.n_positions = p->n_positions;
     w.rope.stride = p->rope_stride; w.rope.rotary_dim = p->cos ? p->rotary_dim : 0; w.rope.style = p->rope_style;
+    w.rope.vec = ((uintptr_t)p->cos & 15) == 0 && ((uintptr_t)p->sin & 15) == 0 && p->rope_stride % 4 == 0;
     w.q_norm = (const uint16_t*)p->q_norm; w.k_norm = (const uint16_t*)p->k_norm; w.eps = p->norm_eps;
-    const uint64_t items = (p->n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * L.n_kv_heads;
-    const uint64_t q_items = (p->n_tokens * w.n_q_heads + 32 / w.lanes_per_row - 1) / (32 / w.lanes_per_row);
-    const uint64_t most = items > q_items ? items : q_items;
-    return kv_launch(a->pc->ctrl, w, (most + w.threads / 32 - 1) / (w.threads / 32), scratch, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+    const uint64_t items = (p->n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * (1 + w.q_parts);
+    return kv_launch(a->pc->ctrl, w, items, scratch, sizeof(kv_launch_words_t), (cudaStream_t)stream);
 }
 
 extern "C" int bam_launch_kv_append(bam_array_t a, const bam_kv_layout_t* layout, const bam_kv_append_t* p, void* scratch_dev,
@@ -396,11 +521,11 @@ extern "C" int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout
     w.n_tokens = n_tokens;
     w.lanes_per_row = lanes_of_row(L.chunks);
     const uint64_t warps = (uint64_t)a->pc->ctrl->num_sms * w.min_blocks * (w.threads / 32);
-    w.tokens_per_item = tokens_of_item(n_tokens, L.n_kv_heads, warps);
+    w.tokens_per_item = tokens_of_item(n_tokens, L.n_kv_heads, warps, KV_MAX_LANE_TOKENS);
     w.vec = (on_16(k_out_dev, k_stride[0], k_stride[1]) ? 1u : 0u) | (on_16(v_out_dev, v_stride[0], v_stride[1]) ? 2u : 0u);
     w.slots = slots_dev;
     const uint64_t items = (n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * L.n_kv_heads;
-    return kv_launch(a->pc->ctrl, w, (items + w.threads / 32 - 1) / (w.threads / 32), scratch_dev, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+    return kv_launch(a->pc->ctrl, w, items, scratch_dev, sizeof(kv_launch_words_t), (cudaStream_t)stream);
 }
 
 extern "C" int bam_launch_kv_attend(bam_array_t a, const bam_kv_layout_t* layout, const bam_kv_attend_t* p, void* scratch_dev,

@@ -27,13 +27,14 @@ namespace bam {
                                        * block uses, a thread may have 255 registers */
 
 /* A launch's own words at the head of its scratch, all ones when the launch starts (one memset, so a captured
- * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks.
- * An index outside its range is noted in `bad` and goes into the status block by the last worker block: a status
- * that is set earlier makes every wait of the launch give up, and a page whose fetch is given up is lost to the cache. */
+ * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks down.
+ * An index outside its range is noted in `bad_index`, bit 31 of `done` tells of it, and it goes into the status block by
+ * the last worker block: a status that is set earlier makes every wait of the launch give up, and a page whose fetch is
+ * given up is lost to the cache. */
 struct kv_launch_words_t {
-    uint32_t remaining, done, bad, pad0;
+    uint32_t remaining, done;
     uint64_t bad_index;
-    uint32_t pad[10];
+    uint32_t pad[12];
 };
 
 /* what a kernel knows of the layout */
@@ -45,7 +46,11 @@ struct kv_layout_d_t {
     uint32_t swz_shift, swz_mask;    /* see swizzle                                           */
     kv_launch_words_t* words;
 
-    BAM_DEV void bad_index(uint64_t i) const { if (atom_cas_relaxed(&words->bad, 0xffffffffu, 1u) == 0xffffffffu) words->bad_index = i; }
+    BAM_DEV void bad_index(uint64_t i) const
+    {
+        st_relaxed_gpu(&words->bad_index, i);
+        (void)atom_and_release(&words->done, 0x7fffffffu);
+    }
     BAM_DEV uint64_t page_of(uint64_t block, uint32_t head) const { return first_page + block * n_kv_heads + head; }
     BAM_DEV uint32_t row_bytes() const { return head_dim * 2u; }
     BAM_DEV uint32_t v_offset() const { return block_tokens * head_dim * 2u; }
@@ -107,7 +112,7 @@ BAM_DEV void kv_store8(uint16_t* p, uint4 v, bool vec)
 
 /* The fused launch of these operators.  Like bam_fused, but the words that end the controller blocks belong to
  * the launch and not to the controller, so that launches on one controller may overlap and a captured launch can
- * be replayed: worker blocks count up from all-ones, and the last one clears `remaining`. */
+ * be replayed: worker blocks count down from all-ones, and the last one clears `remaining`. */
 template <class Work>
 __global__ void __launch_bounds__(Work::threads, Work::min_blocks)
 bam_kv_fused(const __grid_constant__ bam_emu_d_t emu, const __grid_constant__ Work work)
@@ -120,10 +125,14 @@ bam_kv_fused(const __grid_constant__ bam_emu_d_t emu, const __grid_constant__ Wo
     work(blockIdx.x - emu.n_ctrl_blocks, n_work);
     __syncthreads();
     if (threadIdx.x == 0) {
+        /* nothing is published here: what the launch wrote becomes visible with its end */
         kv_launch_words_t* w = reinterpret_cast<kv_launch_words_t*>(emu.consumers_remaining);
-        __threadfence();
-        if (atom_add_acq_rel(&w->done, 1u) == n_work - 2u) {
-            if (ld_relaxed_gpu(&w->bad) == 1u) status_fail(emu.status, BAM_ERANGE, BAM_AT_RANGE, ld_relaxed_gpu(&w->bad_index));
+        const uint32_t left = atom_add_relaxed(&w->done, 0xffffffffu);
+        if ((left & 0x7fffffffu) == 0x80000000u - n_work) {                       /* the last of them */
+            if (!(left & 0x80000000u)) {
+                fence_acq_rel_gpu();
+                status_fail(emu.status, BAM_ERANGE, BAM_AT_RANGE, ld_relaxed_gpu(&w->bad_index));
+            }
             st_release_scoped(&w->remaining, 0u, emu.sys_scope != 0);
         }
     }
@@ -174,8 +183,10 @@ int kv_launch(bam_ctrl* c, const Work& work, uint64_t want, void* scratch, size_
     if (c->max_grid && grid > c->max_grid) grid = c->max_grid;
     bam_emu_d_t emu = c->emu;
     if (want == 0) want = 1;
-    /* few workers need few command processors, and a small grid starts and ends sooner */
-    if (emu.n_ctrl_blocks > 4 && emu.n_ctrl_blocks > want) emu.n_ctrl_blocks = want > 4 ? (uint32_t)want : 4u;
+    /* few workers need few command processors, but one for each queue: a processor that polls several of them in turn
+     * sees the end of the launch a round trip later for each */
+    const uint64_t few = want > (emu.n_qps + BAM_EMU_WARPS - 1) / BAM_EMU_WARPS ? want : (emu.n_qps + BAM_EMU_WARPS - 1) / BAM_EMU_WARPS;
+    if (emu.n_ctrl_blocks > few) emu.n_ctrl_blocks = (uint32_t)few;
     if (grid <= emu.n_ctrl_blocks) return BAM_EINVAL;
     if (grid - emu.n_ctrl_blocks > want) grid = emu.n_ctrl_blocks + (uint32_t)want;
     emu.consumers_remaining = reinterpret_cast<uint32_t*>(scratch);

@@ -151,7 +151,7 @@ struct KvAttendWork {
 
     /* ---- the list ------------------------------------------------------------------------------------- */
     /* how far a cut between two workers moves to fall on the edge of a unit: a join costs what two chunks do */
-    BAM_DEV static uint64_t slack(uint64_t per) { return per / 4 < 2 ? per / 4 : 2; }
+    BAM_DEV static uint64_t slack(uint64_t per) { return per / 8 < 2 ? per / 8 : 2; }
 
     /* The cut before worker i: chunk i * per, or the edge of its unit if that is near.  All lanes. */
     BAM_DEV kv_place_t cut(const kv_shared_t& sh, uint64_t i, uint64_t per, uint64_t total) const

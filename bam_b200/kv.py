@@ -109,7 +109,8 @@ class KvCache:
     def append(self, k, v, slots, layer=0, positions=None, rope=None, rope_style="half", q=None, q_norm=None, k_norm=None,
                norm_eps=1e-6, q_out=None, stream=None):
         """Write the rows k[t], v[t] ([n, n_kv_heads, head_dim], any strides of tokens and heads) to slots[t] (int64;
-        negative: a padding row, nothing is written).  A slot that appears twice keeps either row.
+        negative: a padding row, nothing is written).  The other slots must be distinct: of two rows for one slot neither
+        is sure to be kept whole.
 
         With `k_norm` ([head_dim], of the cache's dtype) every head of k is normed by its root mean square and scaled;
         with `rope` = (cos, sin), float tensors [n_positions, rotary_dim / 2], its first rotary_dim elements are then

@@ -378,8 +378,8 @@ typedef struct {
 } bam_kv_layout_t;
 uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* layout);
 
-/* Append: row t of k and v goes to slots[t] (int64; negative: the row is padding and nothing is written; a slot that
- * appears twice keeps either row).  On the way each head of k, and of q where it is given, is
+/* Append: row t of k and v goes to slots[t] (int64; negative: the row is padding and nothing is written; slots are
+ * distinct otherwise: of two rows for one slot neither is sure to be kept whole).  On the way each head of k, and of q where it is given, is
  *   normed:   y = x * rsqrt(mean(x^2) + norm_eps) * w      (q_norm / k_norm: head_dim elements of the layout's type, or NULL)
  *   rotated:  (a, b) -> (a c - b s, b c + a s) over the first rotary_dim (a multiple of 16) elements, with c and s the
  *             floats cos / sin[positions[t] * rope_stride + i] of pair i (cos NULL: no rotation; positions int64, below
