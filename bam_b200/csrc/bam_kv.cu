@@ -27,7 +27,6 @@ struct kv_rope_d_t {
     int64_t stride;
     uint32_t rotary_dim;         /* 0: no rotation                                             */
     uint32_t style;              /* BAM_KV_ROPE_HALF / BAM_KV_ROPE_PAIRS                       */
-    uint32_t vec;                /* rows of cos and sin lie on 16-byte boundaries               */
 };
 
 /* A lane holds two 16-byte chunks of a row: the two halves of eight rotated pairs where there are such (chunks j and
@@ -37,7 +36,7 @@ struct kv_lane_t {
     uint32_t ca, cb;             /* the lane's chunks; ca = 0xffffffff: none                    */
     bool turned;                 /* they hold rotated pairs                                     */
     float c[8], s[8];            /* of the token at hand                                        */
-    uint4 wa, wb;                /* the norm's weights, of the item at hand                     */
+    float w[16];                 /* the norm's weights, of the item at hand                     */
 };
 
 BAM_DEV kv_lane_t kv_lane(uint32_t j, uint32_t chunks, const kv_rope_d_t& rope)
@@ -49,15 +48,16 @@ BAM_DEV kv_lane_t kv_lane(uint32_t j, uint32_t chunks, const kv_rope_d_t& rope)
     else { n.ca = 2 * j; n.cb = 2 * j + 1; }                           /* rotary_dim and head_dim are multiples of 16 */
     if (n.cb >= chunks) n.ca = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 8; i++) { n.c[i] = 1.f; n.s[i] = 0.f; }
+    for (int i = 0; i < 8; i++) { n.c[i] = 1.f; n.s[i] = 0.f; n.w[i] = n.w[8 + i] = 1.f; }
     return n;
 }
+template <bool VEC>
 BAM_DEV void kv_load_angle(kv_lane_t& n, uint32_t j, const kv_rope_d_t& rope, int64_t pos)
 {
     if (!n.turned || n.ca == 0xffffffffu) return;
     const float* c = rope.cos + pos * rope.stride + j * 8;
     const float* s = rope.sin + pos * rope.stride + j * 8;
-    if (rope.vec) {
+    if (VEC) {
         const float4 c0 = __ldg(reinterpret_cast<const float4*>(c)), c1 = __ldg(reinterpret_cast<const float4*>(c) + 1);
         const float4 s0 = __ldg(reinterpret_cast<const float4*>(s)), s1 = __ldg(reinterpret_cast<const float4*>(s) + 1);
         n.c[0] = c0.x; n.c[1] = c0.y; n.c[2] = c0.z; n.c[3] = c0.w; n.c[4] = c1.x; n.c[5] = c1.y; n.c[6] = c1.z; n.c[7] = c1.w;
@@ -71,7 +71,7 @@ BAM_DEV void kv_load_angle(kv_lane_t& n, uint32_t j, const kv_rope_d_t& rope, in
 /* y = x * rsqrt(mean(x^2) + eps) * w of the row that G lanes hold, then the rotation: in 32 bits, rounded once.  All
  * lanes of the warp call it. */
 template <class T>
-BAM_DEV void kv_transform(uint4& a, uint4& b, const kv_lane_t& n, uint32_t G, uint32_t head_dim, bool norm, float eps,
+BAM_DEV void kv_transform(uint4& a, uint4& b, const kv_lane_t& n, uint32_t G, float inv_dim, bool norm, float eps,
                           const kv_rope_d_t& rope)
 {
     if (!norm && rope.rotary_dim == 0) return;
@@ -89,16 +89,9 @@ BAM_DEV void kv_transform(uint4& a, uint4& b, const kv_lane_t& n, uint32_t G, ui
 #pragma unroll
         for (int i = 0; i < 8; i++) ss += x[i] * x[i] + y[i] * y[i];
         for (uint32_t o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss / (float)head_dim + eps);
-        if (n.ca != 0xffffffffu) {
-            const uint32_t w[8] = { n.wa.x, n.wa.y, n.wa.z, n.wa.w, n.wb.x, n.wb.y, n.wb.z, n.wb.w };
+        const float inv = rsqrtf(ss * inv_dim + eps);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 f = kv_type<T>::unpack(w[i]), g = kv_type<T>::unpack(w[4 + i]);
-                x[2 * i] = x[2 * i] * inv * f.x; x[2 * i + 1] = x[2 * i + 1] * inv * f.y;
-                y[2 * i] = y[2 * i] * inv * g.x; y[2 * i + 1] = y[2 * i + 1] * inv * g.y;
-            }
-        }
+        for (int i = 0; i < 8; i++) { x[i] = x[i] * inv * n.w[i]; y[i] = y[i] * inv * n.w[8 + i]; }
     }
     if (n.turned) {
         if (rope.style == BAM_KV_ROPE_HALF) {
@@ -143,7 +136,11 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
         __syncwarp();
         /* one release per page: the lowest of the lanes that share it gives all their counts back */
         const uint32_t same = __match_any_sync(full, got ? slot : ~lane);
-        if (got && lane == (uint32_t)(__ffs(same) - 1)) L.r.release_page(slot, __popc(same));
+        if (got && lane == (uint32_t)(__ffs(same) - 1)) {
+            /* rows that were read are in registers, or stored from there: there is nothing a release would have to wait for */
+            if (write) L.r.release_page(slot, __popc(same));
+            else red_add_relaxed(&L.r.cache.slots[slot].state, 0u - (uint32_t)__popc(same));
+        }
         if (failed) return false;
         if (got) pending = false;
         if (m == 0u && __any_sync(full, sp.expired(L.r.cache.status, BAM_AT_FIND_SLOT, page))) return false;
@@ -151,16 +148,19 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
     return true;
 }
 
-/* The work is cut into items of tokens_per_item consecutive tokens: KV_Q_HEADS of their query heads, or the keys and values
- * of the runs that begin there.  A run is the tokens in a row that go to one block: one warp writes it, to the end of the
- * run and not of the item, and pins each head's page once.  (Warps that miss the same page at once claim a slot each: a
- * prompt whose pages were written by two warps each evicted half of a cache that had room for all of it.)  Bytes bound it (every row is read and
- * written once); what it needs for that is rows in flight: KV_ROWS_AHEAD rows of a lane are loaded before the first is
- * worked on, and angles are loaded once per token and item. */
+/* The work is cut into items that warps draw in turn: first KV_K_HEADS of the key/value heads of the runs that begin in k_tokens
+ * consecutive tokens, then KV_Q_HEADS of the query heads of q_tokens tokens.  A run is the tokens in a row that go to one
+ * block: one warp writes its share of it, to the end of the run and not of the item, and pins each page once.  (Warps that
+ * miss the same page at once claim a slot each: a prompt whose pages were written by two warps each evicted half of a cache
+ * with room for all.)  Items differ in length, hence the drawing; which warp writes a row changes nothing in it.
+ * Bytes bound it, every row is read and written once; what that needs is rows in flight: several rows of a lane are loaded
+ * before the first is worked on.  Angles are loaded once per token and item for the queries. */
 #define KV_Q_HEADS 16u
+#define KV_K_HEADS 2u
 #define KV_ROWS_AHEAD 4
 
-template <class T>
+/* VEC: every row, weight and angle lies on a 16-byte boundary. */
+template <class T, bool VEC>
 struct KvAppendWork {
     static constexpr int threads = BAM_THREADS, min_blocks = 2;
     static constexpr uint32_t smem = BAM_FUSED_SMEM;
@@ -169,12 +169,11 @@ struct KvAppendWork {
     uint16_t* q_out;
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh;      /* element strides of token and head */
     uint64_t n_tokens;
-    uint32_t n_q_heads, lanes_per_row, tokens_per_item, q_parts;
-    uint32_t vec;                                                  /* bit 0: q, 1: k, 2: v, 3: q_out, 4: q_norm, 5: k_norm lie on 16-byte boundaries */
+    uint32_t n_q_heads, lanes_per_row, k_tokens, q_tokens, k_parts, q_parts;
     const int64_t* slots;
     kv_rope_d_t rope;
     const uint16_t *q_norm, *k_norm;
-    float eps;
+    float eps, inv_dim;
 
     /* the position of a token, or -1 after the error has been recorded */
     BAM_DEV int64_t position(uint64_t t, bool padded) const
@@ -209,56 +208,61 @@ struct KvAppendWork {
                 const uint32_t r = r0 + i * rows + grp;
                 a[i] = b[i] = make_uint4(0, 0, 0, 0);
                 if (r < n && ln.ca != 0xffffffffu) {
-                    a[i] = kv_load8(src + (h0 + r) * q_sh + ln.ca * 8, vec & 1u);
-                    b[i] = kv_load8(src + (h0 + r) * q_sh + ln.cb * 8, vec & 1u);
+                    a[i] = kv_load8(src + (h0 + r) * q_sh + ln.ca * 8, VEC);
+                    b[i] = kv_load8(src + (h0 + r) * q_sh + ln.cb * 8, VEC);
                 }
             }
 #pragma unroll
             for (int i = 0; i < KV_ROWS_AHEAD; i++) {
                 if (r0 + i * rows >= n) break;
                 const uint32_t r = r0 + i * rows + grp;
-                kv_transform<T>(a[i], b[i], ln, G, L.head_dim, q_norm != nullptr, eps, rope);
+                kv_transform<T>(a[i], b[i], ln, G, inv_dim, q_norm != nullptr, eps, rope);
                 if (r < n && ln.ca != 0xffffffffu) {
-                    kv_store8(dst + (h0 + r) * qo_sh + ln.ca * 8, a[i], vec & 8u);
-                    kv_store8(dst + (h0 + r) * qo_sh + ln.cb * 8, b[i], vec & 8u);
+                    kv_store8(dst + (h0 + r) * qo_sh + ln.ca * 8, a[i], VEC);
+                    kv_store8(dst + (h0 + r) * qo_sh + ln.cb * 8, b[i], VEC);
                 }
             }
         }
     }
 
-    /* keys and values of one token into row `row` of the pages at `addr` (lane: head h0 + lane, those of mask m) */
-    BAM_DEV void keys(uint64_t t, uint32_t row, uint32_t h0, uint32_t n, uint32_t m, uint64_t addr, const kv_lane_t& ln, uint32_t G, uint32_t grp) const
+    /* Keys and values of the tokens t1 + i, i in `run` (a mask of the first n_run), heads h0 .. h0 + nh of them whose pages
+     * are there (lane h of mask m holds the page of head h0 + h; lane i the row and the position of token i). */
+    BAM_DEV void keys(uint64_t t1, uint32_t run, uint32_t n_run, uint32_t h0, uint32_t nh, uint32_t m, uint64_t addr, uint32_t row, int64_t pos,
+                      const kv_lane_t& item, uint32_t j, uint32_t G, uint32_t grp) const
     {
-        const uint32_t rows = 32u / G;
-        const uint16_t *ks = k + (int64_t)t * k_st, *vs = v + (int64_t)t * v_st;
-        const uint32_t oa = row * L.row_bytes() + L.swizzle(row, ln.ca) * 16u, ob = row * L.row_bytes() + L.swizzle(row, ln.cb) * 16u;
-        for (uint32_t r0 = 0; r0 < n; r0 += rows * 2) {
-            uint4 ka[2], kb[2], va[2], vb[2];
-            uint64_t page[2];
-            bool act[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t r = r0 + i * rows + grp;
-                page[i] = __shfl_sync(0xffffffffu, addr, r & 31u);
-                act[i] = r < n && ((m >> (r & 31u)) & 1u) && ln.ca != 0xffffffffu;
-                ka[i] = kb[i] = va[i] = vb[i] = make_uint4(0, 0, 0, 0);
-                if (act[i]) {
-                    ka[i] = kv_load8(ks + (h0 + r) * k_sh + ln.ca * 8, vec & 2u);
-                    kb[i] = kv_load8(ks + (h0 + r) * k_sh + ln.cb * 8, vec & 2u);
-                    va[i] = kv_load8(vs + (h0 + r) * v_sh + ln.ca * 8, vec & 4u);
-                    vb[i] = kv_load8(vs + (h0 + r) * v_sh + ln.cb * 8, vec & 4u);
-                }
+        const uint32_t full = 0xffffffffu, rows = 32u / G, n = n_run * nh;
+        /* row r: token r / nh, head r % nh */
+        auto place = [&](uint32_t r, uint32_t& i, uint32_t& h, uint8_t*& base, uint32_t& rr) {
+            i = r / nh;
+            h = r - i * nh;
+            base = reinterpret_cast<uint8_t*>(__shfl_sync(full, addr, h & 31u));
+            rr = __shfl_sync(full, row, i & 31u);
+            return r < n && ((run >> (i & 31u)) & 1u) && ((m >> (h & 31u)) & 1u) && item.ca != 0xffffffffu;
+        };
+        kv_lane_t ln = item;
+        for (uint32_t r0 = 0; r0 < n; r0 += rows) {                                  /* every row has its token's angles */
+            uint32_t i, h, rr;
+            uint8_t* dst;
+            if (!place(r0 + grp, i, h, dst, rr)) dst = nullptr;
+            const int64_t at = __shfl_sync(full, pos, i & 31u);
+            uint4 a = make_uint4(0, 0, 0, 0), b = a, va = a, vb = a;
+            if (dst) {
+                const uint16_t* src = k + (int64_t)(t1 + i) * k_st + (h0 + h) * k_sh;
+                a = kv_load8(src + item.ca * 8, VEC);
+                b = kv_load8(src + item.cb * 8, VEC);
+                kv_load_angle<VEC>(ln, j, rope, at);
+                src = v + (int64_t)(t1 + i) * v_st + (h0 + h) * v_sh;
+                va = kv_load8(src + item.ca * 8, VEC);
+                vb = kv_load8(src + item.cb * 8, VEC);
             }
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                kv_transform<T>(ka[i], kb[i], ln, G, L.head_dim, k_norm != nullptr, eps, rope);
-                if (act[i]) {
-                    uint8_t* p = reinterpret_cast<uint8_t*>(page[i]);
-                    *reinterpret_cast<uint4*>(p + oa) = ka[i];
-                    *reinterpret_cast<uint4*>(p + ob) = kb[i];
-                    *reinterpret_cast<uint4*>(p + L.v_offset() + oa) = va[i];
-                    *reinterpret_cast<uint4*>(p + L.v_offset() + ob) = vb[i];
-                }
+            kv_transform<T>(a, b, ln, G, inv_dim, k_norm != nullptr, eps, rope);
+            if (dst) {
+                uint8_t* p = dst + rr * L.row_bytes() + L.swizzle(rr, item.ca) * 16u;
+                *reinterpret_cast<uint4*>(p) = a;
+                *reinterpret_cast<uint4*>(p + L.v_offset()) = va;
+                p = dst + rr * L.row_bytes() + L.swizzle(rr, item.cb) * 16u;
+                *reinterpret_cast<uint4*>(p) = b;
+                *reinterpret_cast<uint4*>(p + L.v_offset()) = vb;
             }
         }
     }
@@ -270,23 +274,29 @@ struct KvAppendWork {
         const uint32_t G = lanes_per_row, j = lane & (G - 1u), grp = lane / G;
         if (status_bad(L.r.cache.status)) return;
         kv_lane_t ln = kv_lane(j, L.chunks, rope);
-        const uint64_t groups = (n_tokens + tokens_per_item - 1) / tokens_per_item;
-        for (uint64_t it = warp; it < groups * (1 + q_parts); it += nwarps) {
-            const uint32_t part = (uint32_t)(it % (1 + q_parts));
-            const uint64_t t0 = it / (1 + q_parts) * tokens_per_item;
-            const uint32_t nt = n_tokens - t0 < tokens_per_item ? (uint32_t)(n_tokens - t0) : tokens_per_item;
-            const uint16_t* norm = part ? q_norm : k_norm;
+        const uint64_t k_items = (n_tokens + k_tokens - 1) / k_tokens * k_parts;
+        const uint64_t n_items = k_items + (q_parts ? (n_tokens + q_tokens - 1) / q_tokens * q_parts : 0u);
+        for (uint64_t it = warp; it < n_items; it = nwarps + L.draw()) {
+            const bool queries_of = it >= k_items;
+            const uint64_t x = queries_of ? it - k_items : it;
+            const uint32_t parts = queries_of ? q_parts : k_parts, span = queries_of ? q_tokens : k_tokens;
+            const uint32_t part = (uint32_t)(x % parts);
+            const uint64_t t0 = x / parts * span;
+            const uint32_t nt = n_tokens - t0 < span ? (uint32_t)(n_tokens - t0) : span;
+            const uint16_t* norm = queries_of ? q_norm : k_norm;
             if (norm && ln.ca != 0xffffffffu) {
-                ln.wa = kv_load8(norm + ln.ca * 8, vec & (part ? 16u : 32u));
-                ln.wb = kv_load8(norm + ln.cb * 8, vec & (part ? 16u : 32u));
+                const uint4 wa = kv_load8(norm + ln.ca * 8, VEC), wb = kv_load8(norm + ln.cb * 8, VEC);
+                const uint32_t w[8] = { wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w };
+#pragma unroll
+                for (int i = 0; i < 8; i++) { const float2 f = kv_type<T>::unpack(w[i]); ln.w[2 * i] = f.x; ln.w[2 * i + 1] = f.y; }
             }
-            if (part) {
-                const uint32_t h0 = (part - 1) * KV_Q_HEADS, n = n_q_heads - h0 < KV_Q_HEADS ? n_q_heads - h0 : KV_Q_HEADS;
+            if (queries_of) {
+                const uint32_t h0 = part * KV_Q_HEADS, n = n_q_heads - h0 < KV_Q_HEADS ? n_q_heads - h0 : KV_Q_HEADS;
                 const int64_t pos = lane < nt ? position(t0 + lane, slots[t0 + lane] < 0) : 0;
                 for (uint32_t i = 0; i < nt; i++) {
                     const int64_t p = __shfl_sync(full, pos, i);
                     if (p < 0) continue;
-                    kv_load_angle(ln, j, rope, p);
+                    kv_load_angle<VEC>(ln, j, rope, p);
                     queries(t0 + i, h0, n, ln, G, grp);
                 }
                 continue;
@@ -305,17 +315,10 @@ struct KvAppendWork {
                     const int64_t pos = live ? position(t, false) : 0;
                     const uint32_t row = live ? (uint32_t)((uint64_t)slots[t] % L.block_tokens) : 0;
                     const uint32_t run = in_run & __ballot_sync(full, pos >= 0);
-                    for (uint32_t h0 = 0; h0 < L.n_kv_heads && run; h0 += 32) {
-                        const uint32_t n = L.n_kv_heads - h0 < 32u ? L.n_kv_heads - h0 : 32u;
-                        const bool ok = kv_with_pages(L, lane < n, L.page_of(at, h0 + lane), true, (uint32_t)warp, [&](uint32_t m, uint64_t addr) {
-                            for (uint32_t left = run; left; left &= left - 1) {
-                                const uint32_t i = __ffs(left) - 1;
-                                kv_load_angle(ln, j, rope, __shfl_sync(full, pos, i));
-                                keys(t1 + i, __shfl_sync(full, row, i), h0, n, m, addr, ln, G, grp);
-                            }
-                        });
-                        if (!ok) return;
-                    }
+                    const uint32_t h0 = part * KV_K_HEADS, nh = L.n_kv_heads - h0 < KV_K_HEADS ? L.n_kv_heads - h0 : KV_K_HEADS;
+                    if (run && !kv_with_pages(L, lane < nh, L.page_of(at, h0 + lane), true, (uint32_t)warp, [&](uint32_t m, uint64_t addr) {
+                            keys(t1, run, 32u - __clz(run), h0, nh, m, addr, row, pos, ln, j, G, grp);
+                        })) return;
                     if (gap) break;
                 }
             }
@@ -327,15 +330,15 @@ struct KvAppendWork {
 /* gather                                                                                  */
 /* ====================================================================================== */
 
+template <bool VEC>
 struct KvGatherWork {
-    static constexpr int threads = BAM_THREADS, min_blocks = 2;
+    static constexpr int threads = BAM_THREADS, min_blocks = 3;
     static constexpr uint32_t smem = BAM_FUSED_SMEM;
     kv_layout_d_t L;
     uint16_t *k, *v;
     int64_t k_st, k_sh, v_st, v_sh;
     uint64_t n_tokens;
     uint32_t lanes_per_row, tokens_per_item;
-    uint32_t vec;
     const int64_t* slots;
 
     __device__ void operator()(uint32_t vb, uint32_t nvb) const
@@ -346,7 +349,7 @@ struct KvGatherWork {
         const bool in_row = c < L.chunks;
         if (status_bad(L.r.cache.status)) return;
         const uint64_t groups = (n_tokens + tokens_per_item - 1) / tokens_per_item;
-        for (uint64_t it = warp; it < groups * L.n_kv_heads; it += nwarps) {
+        for (uint64_t it = warp; it < groups * L.n_kv_heads; it = nwarps + L.draw()) {
             const uint32_t h = (uint32_t)(it % L.n_kv_heads);
             const uint64_t t0 = it / L.n_kv_heads * tokens_per_item;
             const uint64_t t = t0 + lane;
@@ -380,8 +383,8 @@ struct KvGatherWork {
                     for (int e = 0; e < KV_ROWS_AHEAD; e++) {
                         const uint32_t i = i0 + e * rows, src = (i + grp) & 31u;
                         if (in_row && i + grp < tokens_per_item && ((m >> src) & 1u)) {
-                            kv_store8(k + (int64_t)(t0 + src) * k_st + h * k_sh + c * 8, kk[e], vec & 1u);
-                            kv_store8(v + (int64_t)(t0 + src) * v_st + h * v_sh + c * 8, vv[e], vec & 2u);
+                            kv_store8(k + (int64_t)(t0 + src) * k_st + h * k_sh + c * 8, kk[e], VEC);
+                            kv_store8(v + (int64_t)(t0 + src) * v_st + h * v_sh + c * 8, vv[e], VEC);
                         }
                     }
                 }
@@ -426,8 +429,7 @@ uint32_t lanes_of_row(uint32_t chunks) { uint32_t g = 1; while (g < chunks) g <<
 
 bool on_16(const void* p, int64_t s0, int64_t s1) { return ((uintptr_t)p & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0; }
 
-/* tokens a warp takes at a time: as many (up to `most`) as leave every warp of the GPU something to do.  Tokens of one
- * block that go to different warps pin its page each, so they are kept together where that costs no parallelism. */
+/* tokens a warp takes at a time: as many (up to `most`) as still make an item for every warp */
 uint32_t tokens_of_item(uint64_t n_tokens, uint32_t parts, uint64_t warps, uint32_t most)
 {
     uint32_t t = most;
@@ -451,10 +453,10 @@ static int check_scratch(bam_array_t a, const bam_kv_layout_t* layout, void* scr
     return scratch_bytes < bam_kv_scratch_bytes(a, layout) ? BAM_EINVAL : BAM_OK;
 }
 
-template <class T>
-static int launch_append(bam_array_t a, const kv_layout_d_t& L, const bam_kv_append_t* p, void* scratch, void* stream)
+template <class T, bool VEC>
+static int launch_append_as(bam_array_t a, const kv_layout_d_t& L, const bam_kv_append_t* p, void* scratch, void* stream)
 {
-    KvAppendWork<T> w;
+    KvAppendWork<T, VEC> w;
     memset(&w, 0, sizeof w);
     w.L = L;
     w.q = (const uint16_t*)p->q; w.k = (const uint16_t*)p->k; w.v = (const uint16_t*)p->v; w.q_out = (uint16_t*)p->q_out;
@@ -462,19 +464,26 @@ static int launch_append(bam_array_t a, const kv_layout_d_t& L, const bam_kv_app
     w.v_st = p->v_stride[0]; w.v_sh = p->v_stride[1]; w.qo_st = p->q_out_stride[0]; w.qo_sh = p->q_out_stride[1];
     w.n_tokens = p->n_tokens; w.n_q_heads = p->q ? p->n_q_heads : 0;
     w.lanes_per_row = lanes_of_row(L.chunks / 2);
+    w.k_parts = (L.n_kv_heads + KV_K_HEADS - 1) / KV_K_HEADS;
     w.q_parts = (w.n_q_heads + KV_Q_HEADS - 1) / KV_Q_HEADS;
     const uint64_t warps = (uint64_t)a->pc->ctrl->num_sms * w.min_blocks * (w.threads / 32);
-    w.tokens_per_item = tokens_of_item(p->n_tokens, 1 + w.q_parts, warps, 16);
-    w.vec = (on_16(p->q, p->q_stride[0], p->q_stride[1]) ? 1u : 0u) | (on_16(p->k, p->k_stride[0], p->k_stride[1]) ? 2u : 0u) |
-            (on_16(p->v, p->v_stride[0], p->v_stride[1]) ? 4u : 0u) | (on_16(p->q_out, p->q_out_stride[0], p->q_out_stride[1]) ? 8u : 0u) |
-            (on_16(p->q_norm, 0, 0) ? 16u : 0u) | (on_16(p->k_norm, 0, 0) ? 32u : 0u);
+    w.k_tokens = tokens_of_item(p->n_tokens, w.k_parts, warps, 32);
+    w.q_tokens = tokens_of_item(p->n_tokens, w.q_parts, 2 * warps, 16);
     w.slots = p->slots;
     w.rope.positions = p->positions; w.rope.cos = p->cos; w.rope.sin = p->sin; w.rope.n_positions = p->n_positions;
     w.rope.stride = p->rope_stride; w.rope.rotary_dim = p->cos ? p->rotary_dim : 0; w.rope.style = p->rope_style;
-    w.rope.vec = ((uintptr_t)p->cos & 15) == 0 && ((uintptr_t)p->sin & 15) == 0 && p->rope_stride % 4 == 0;
-    w.q_norm = (const uint16_t*)p->q_norm; w.k_norm = (const uint16_t*)p->k_norm; w.eps = p->norm_eps;
-    const uint64_t items = (p->n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * (1 + w.q_parts);
+    w.q_norm = (const uint16_t*)p->q_norm; w.k_norm = (const uint16_t*)p->k_norm; w.eps = p->norm_eps; w.inv_dim = 1.f / (float)L.head_dim;
+    const uint64_t items = (p->n_tokens + w.k_tokens - 1) / w.k_tokens * w.k_parts + (p->n_tokens + w.q_tokens - 1) / w.q_tokens * w.q_parts;
     return kv_launch(a->pc->ctrl, w, items, scratch, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+}
+
+template <class T>
+static int launch_append(bam_array_t a, const kv_layout_d_t& L, const bam_kv_append_t* p, void* scratch, void* stream)
+{
+    const bool vec = (!p->q || (on_16(p->q, p->q_stride[0], p->q_stride[1]) && on_16(p->q_out, p->q_out_stride[0], p->q_out_stride[1]))) &&
+                     on_16(p->k, p->k_stride[0], p->k_stride[1]) && on_16(p->v, p->v_stride[0], p->v_stride[1]) && on_16(p->q_norm, 0, 0) &&
+                     on_16(p->k_norm, 0, 0) && on_16(p->cos, 2 * p->rope_stride, 0) && on_16(p->sin, 2 * p->rope_stride, 0);
+    return vec ? launch_append_as<T, true>(a, L, p, scratch, stream) : launch_append_as<T, false>(a, L, p, scratch, stream);
 }
 
 extern "C" int bam_launch_kv_append(bam_array_t a, const bam_kv_layout_t* layout, const bam_kv_append_t* p, void* scratch_dev,
@@ -500,6 +509,24 @@ extern "C" int bam_launch_kv_append(bam_array_t a, const bam_kv_layout_t* layout
                                         : launch_append<__half>(a, L, p, scratch_dev, stream);
 }
 
+template <bool VEC>
+static int launch_gather(bam_array_t a, const kv_layout_d_t& L, uint64_t n_tokens, const int64_t* slots_dev, void* k_out_dev, void* v_out_dev,
+                         const int64_t* k_stride, const int64_t* v_stride, void* scratch, void* stream)
+{
+    KvGatherWork<VEC> w;
+    memset(&w, 0, sizeof w);
+    w.L = L;
+    w.k = (uint16_t*)k_out_dev; w.v = (uint16_t*)v_out_dev;
+    w.k_st = k_stride[0]; w.k_sh = k_stride[1]; w.v_st = v_stride[0]; w.v_sh = v_stride[1];
+    w.n_tokens = n_tokens;
+    w.lanes_per_row = lanes_of_row(L.chunks);
+    const uint64_t warps = (uint64_t)a->pc->ctrl->num_sms * w.min_blocks * (w.threads / 32);
+    w.tokens_per_item = tokens_of_item(n_tokens, L.n_kv_heads, warps, KV_MAX_LANE_TOKENS);
+    w.slots = slots_dev;
+    const uint64_t items = (n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * L.n_kv_heads;
+    return kv_launch(a->pc->ctrl, w, items, scratch, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+}
+
 extern "C" int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t n_tokens, const int64_t* slots_dev,
                                     void* k_out_dev, void* v_out_dev, const int64_t* k_stride, const int64_t* v_stride,
                                     void* scratch_dev, uint64_t scratch_bytes, void* stream)
@@ -513,19 +540,9 @@ extern "C" int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout
     if (n_tokens == 0) return BAM_OK;
     device_guard g;
     CK(g.enter(a->pc->ctrl->device));
-    KvGatherWork w;
-    memset(&w, 0, sizeof w);
-    w.L = L;
-    w.k = (uint16_t*)k_out_dev; w.v = (uint16_t*)v_out_dev;
-    w.k_st = k_stride[0]; w.k_sh = k_stride[1]; w.v_st = v_stride[0]; w.v_sh = v_stride[1];
-    w.n_tokens = n_tokens;
-    w.lanes_per_row = lanes_of_row(L.chunks);
-    const uint64_t warps = (uint64_t)a->pc->ctrl->num_sms * w.min_blocks * (w.threads / 32);
-    w.tokens_per_item = tokens_of_item(n_tokens, L.n_kv_heads, warps, KV_MAX_LANE_TOKENS);
-    w.vec = (on_16(k_out_dev, k_stride[0], k_stride[1]) ? 1u : 0u) | (on_16(v_out_dev, v_stride[0], v_stride[1]) ? 2u : 0u);
-    w.slots = slots_dev;
-    const uint64_t items = (n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * L.n_kv_heads;
-    return kv_launch(a->pc->ctrl, w, items, scratch_dev, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+    const bool vec = on_16(k_out_dev, k_stride[0], k_stride[1]) && on_16(v_out_dev, v_stride[0], v_stride[1]);
+    return vec ? launch_gather<true>(a, L, n_tokens, slots_dev, k_out_dev, v_out_dev, k_stride, v_stride, scratch_dev, stream)
+               : launch_gather<false>(a, L, n_tokens, slots_dev, k_out_dev, v_out_dev, k_stride, v_stride, scratch_dev, stream);
 }
 
 extern "C" int bam_launch_kv_attend(bam_array_t a, const bam_kv_layout_t* layout, const bam_kv_attend_t* p, void* scratch_dev,

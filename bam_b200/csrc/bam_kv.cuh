@@ -27,14 +27,15 @@ namespace bam {
                                        * block uses, a thread may have 255 registers */
 
 /* A launch's own words at the head of its scratch, all ones when the launch starts (one memset, so a captured
- * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks down.
+ * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks down,
+ * `drawn` counts the items that were drawn.
  * An index outside its range is noted in `bad_index`, bit 31 of `done` tells of it, and it goes into the status block by
  * the last worker block: a status that is set earlier makes every wait of the launch give up, and a page whose fetch is
  * given up is lost to the cache. */
 struct kv_launch_words_t {
     uint32_t remaining, done;
     uint64_t bad_index;
-    uint32_t pad[12];
+    uint32_t drawn, pad[11];
 };
 
 /* what a kernel knows of the layout */
@@ -50,6 +51,13 @@ struct kv_layout_d_t {
     {
         st_relaxed_gpu(&words->bad_index, i);
         (void)atom_and_release(&words->done, 0x7fffffffu);
+    }
+    /* the number of draws before this one; a warp draws together */
+    BAM_DEV uint32_t draw() const
+    {
+        uint32_t n = 0;
+        if (lane_id() == 0) n = atom_add_relaxed(&words->drawn, 1u) + 1u;
+        return __shfl_sync(0xffffffffu, n, 0);
     }
     BAM_DEV uint64_t page_of(uint64_t block, uint32_t head) const { return first_page + block * n_kv_heads + head; }
     BAM_DEV uint32_t row_bytes() const { return head_dim * 2u; }
