@@ -12,8 +12,8 @@ namespace bam {
 
 /* The flattened work list: sequence b has `n` chunks of CS tokens with something visible in them, in each of its
  * n_kv_heads * tiles units (a unit: 16 query heads of one key/value head), and the list is b-major, then unit, then
- * chunk.  A WARP is a worker: it takes a run of `per` chunks, copies them into its own stages of shared memory and keeps
- * one running softmax.  Every warp reads the same amount whatever the lengths
+ * chunk.  A WARP is a worker: it takes one of as many equal runs as there are workers, copies their chunks into its own stages of shared memory
+ * and keeps one running softmax.  Every warp reads the same amount whatever the lengths
  * are, a long sequence is split over many warps and a short one is not split at all (cuts that fall next to the edge
  * of a unit move there).  Warps share nothing and wait for nothing of one another until the end: one that does not
  * own a whole unit writes its running maximum, denominator and unnormalised sum to the scratch, and then the warps of
@@ -25,9 +25,11 @@ namespace bam {
  * more chunks under way for each (200 KB of an SM's shared memory).  The fourth warp of a block looks their pages up and
  * pins them up to 16 chunks ahead: a look-up is three dependent accesses that miss L2 while the rows stream through it,
  * 2 to 5 us (done by the workers themselves, 32 pages at a time, it cost 10 us of 186 on the largest case).
- * The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured): 16 query heads are
- * all the rows there are, and a chunk of 32 tokens at 128 dimensions takes 200 of the 710 cycles that HBM needs to
- * deliver it to an SM; the 128-row tcgen05 tiles would be seven eighths padding. */
+ * The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured): up to 16 query heads are
+ * all there is, the 128-row tcgen05 tiles would be seven eighths padding.  The scores have the queries as rows and the sums
+ * as columns, S = Q K^T and O^T = V^T P^T: the scores are then where the second product wants its right operand, and
+ * eight query heads take half of the instructions (and of the registers for O) that sixteen do.  At 128 dimensions a
+ * chunk of 32 tokens takes 64 of them, 130 of the 710 cycles that HBM needs to deliver it to an SM. */
 #define KV_STAGES_MAX 8u              /* stages of a worker */
 #define KV_AHEAD 16u                  /* chunks of a worker that are pinned and not yet consumed, at most */
 #define KV_PIN_LANES 10u              /* lanes of the pinning warp for each worker */
@@ -58,8 +60,11 @@ BAM_DEV void ldm_x4_t(uint32_t (&r)[4], uint32_t addr)
 }
 /* 2^x, off by two units in the last place at most; results below the normal range are 0 */
 BAM_DEV float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+BAM_DEV void st_cg_f4(float* p, float x, float y, float z, float w)
+{
+    asm volatile("st.global.cg.v4.f32 [%0], {%1,%2,%3,%4};" ::"l"(p), "f"(x), "f"(y), "f"(z), "f"(w) : "memory");
+}
 BAM_DEV void st_cg_f2(float* p, float x, float y) { asm volatile("st.global.cg.v2.f32 [%0], {%1,%2};" ::"l"(p), "f"(x), "f"(y) : "memory"); }
-BAM_DEV float2 ld_cg_f2(const float* p) { float2 v; asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory"); return v; }
 
 /* Where a worker's run begins, or a chunk is: sequence, chunk within the sequence's share of the list. */
 struct kv_place_t {
@@ -92,8 +97,8 @@ BAM_DEV void st_release_cta(uint32_t* p, uint32_t v) { asm volatile("st.release.
 
 /* DMAX: the head_dim the registers are laid out for, and with EXACT the head_dim itself (otherwise every step over
  * the dimensions asks whether it is needed, which keeps the compiler from overlapping them: 3 times the time of a
- * chunk at 128); CS: tokens of a chunk. */
-template <class T, int DMAX, int CS, bool EXACT>
+ * chunk at 128); CS: tokens of a chunk; NT: groups of eight query heads in a unit. */
+template <class T, int DMAX, int CS, bool EXACT, int NT>
 struct KvAttendWork {
     static constexpr int threads = 32 * (KV_WORKERS + 1), min_blocks = 2;
     static constexpr uint32_t smem = 112 * 1024;
@@ -150,16 +155,22 @@ struct KvAttendWork {
     BAM_DEV static int64_t first_token(const kv_seen_t& v, uint32_t c) { return (int64_t)(c < v.n_first ? c : v.from + (c - v.n_first)) * CS; }
 
     /* ---- the list ------------------------------------------------------------------------------------- */
-    /* how far a cut between two workers moves to fall on the edge of a unit: a join costs what two chunks do */
-    BAM_DEV static uint64_t slack(uint64_t per) { return per / 8 < 2 ? per / 8 : 2; }
+    /* The list and the workers that share it: worker i takes the chunks from i * total / workers on (all differ by one
+     * chunk at most), but a cut that falls within `slack` chunks of the edge of a unit moves there: a join costs what
+     * two chunks do. */
+    struct list_t {
+        uint64_t total, workers, slack;
+        BAM_DEV uint64_t cut(uint64_t i) const { return i * total / workers; }
+        BAM_DEV uint64_t worker_of(uint64_t x) const { return ((x + 1) * workers - 1) / total; }      /* before cuts move */
+    };
 
-    /* The cut before worker i: chunk i * per, or the edge of its unit if that is near.  All lanes. */
-    BAM_DEV kv_place_t cut(const kv_shared_t& sh, uint64_t i, uint64_t per, uint64_t total) const
+    /* Where worker i's run begins.  All lanes. */
+    BAM_DEV kv_place_t begin_of(const kv_shared_t& sh, uint64_t i, const list_t& list) const
     {
         const uint32_t lane = lane_id(), units = L.n_kv_heads * tiles;
-        const uint64_t x = i * per;
-        kv_place_t p = { total, 0, 0 };
-        if (x >= total) return p;
+        kv_place_t p = { list.total, 0, 0 };
+        if (i >= list.workers) return p;
+        const uint64_t x = list.cut(i);
         uint32_t t = 0;
 #pragma unroll
         for (uint32_t k = 0; k < KV_WORKERS + 1; k++) t += __popc(__ballot_sync(0xffffffffu, sh.before[k * 32 + lane] <= x));
@@ -187,18 +198,18 @@ struct KvAttendWork {
         }
         const uint64_t n = seen(p.b).n, in = (x - at) % n;
         p.f = x;
-        if (in <= slack(per)) p.f = x - in;
-        else if (n - in <= slack(per)) p.f = x + (n - in);
+        if (in <= list.slack) p.f = x - in;
+        else if (n - in <= list.slack) p.f = x + (n - in);
         p.pos = p.f - at;
         return p;
     }
-    /* the first worker of the unit [U0, U1), and how many there are (see cut) */
-    BAM_DEV static void workers_of(uint64_t U0, uint64_t U1, uint64_t per, uint32_t& first, uint32_t& count)
+    /* the first worker of the unit [U0, U1), and how many there are */
+    BAM_DEV static void workers_of(uint64_t U0, uint64_t U1, const list_t& list, uint32_t& first, uint32_t& count)
     {
-        uint64_t i0 = U0 / per, i1 = (U1 - 1) / per;
-        const uint64_t up = (i0 + 1) * per, down = i1 * per;
-        if (up < U1 && up - U0 <= slack(per)) i0++;
-        if (down > U0 && down - U0 > slack(per) && U1 - down <= slack(per)) i1--;
+        uint64_t i0 = list.worker_of(U0), i1 = list.worker_of(U1 - 1);
+        const uint64_t up = list.cut(i0 + 1), down = list.cut(i1);
+        if (up < U1 && up - U0 <= list.slack) i0++;
+        if (down > U0 && down - U0 > list.slack && U1 - down <= list.slack) i1--;
         first = (uint32_t)i0;
         count = (uint32_t)(i1 - i0 + 1);
     }
@@ -394,14 +405,27 @@ struct KvAttendWork {
         for (int i = 0; i < DMAX / 4; i++) a[i >> 2][i & 3] ^= q_sign;
     }
 
+    /* The running softmax.  Thread (r, c) = (lane / 4, lane % 4) holds m and l of queries r and r + 8 (its share of l),
+     * and of the sums the dimensions 16 i + r and + 8 of queries 8 n + 2 c and + 1. */
     struct state_t {
-        float o[DMAX / 8][4];
+        float o[NT][DMAX / 16][4];
         float m[2], l[2];
     };
+    /* what a thread knows of queries lane / 4 and lane / 4 + 8, for the queries of its columns */
+    BAM_DEV static void to_columns(float x0, float x1, float (&c)[NT][2])
+    {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t src = ((lane_id() & 3u) * 2 + e) * 4;
+            c[0][e] = __shfl_sync(0xffffffffu, x0, src);
+            if (NT == 2) c[NT - 1][e] = __shfl_sync(0xffffffffu, x1, src);
+        }
+    }
 
-    /* One chunk: S = Q K^T, p = 2^(S scale log2(e) - m), O += p V.  The weights go into the product as two 16-bit
-     * parts, p = hi + lo, which keeps 16 (bf16) or more bits of them: the product runs twice, on a pipe that idles. */
-    template <bool WHOLE>
+    /* One chunk: S = Q K^T, p = 2^(S scale log2(e) - m), O^T += V^T p^T.  The weights go into the product as two 16-bit
+     * parts, p = hi + lo, which keeps 16 (bf16) or more bits of them: the product runs twice, on a pipe that idles.
+     * There is one copy of this code, for whole chunks and others: code that runs once a unit runs from a cold
+     * instruction cache, at a microsecond for every few kilobytes. */
     BAM_DEV void chunk(state_t& z, const uint32_t (&qa)[DMAX / 16][4], uint32_t stage, const kv_seen_t& v, int64_t t0) const
     {
         const uint32_t lane = lane_id(), rb = row_bytes();
@@ -427,23 +451,27 @@ struct KvAttendWork {
                 }
             }
         }
-        /* bit i: this lane's column i (of its CS / 4) is visible */
-        uint32_t vis = 0;
-        if (!WHOLE) {
+        if (!(t0 + CS <= v.first || (t0 >= v.begin && t0 + CS <= v.len))) {
+            /* rows that are not visible may hold anything.  Their scores become -infinity and their values zeros: their
+             * weights are 0, and 0 x NaN is not 0 */
 #pragma unroll
             for (int i = 0; i < CS / 4; i++) {
                 const int64_t j = t0 + (i >> 1) * 8 + (lane & 3u) * 2 + (i & 1);
-                if ((j < v.first || j >= v.begin) && j < v.len) vis |= 1u << i;
+                if (!((j < v.first || j >= v.begin) && j < v.len)) s[i >> 1][i & 1] = s[i >> 1][2 + (i & 1)] = -INFINITY;
             }
+#pragma unroll 1
+            for (uint32_t i = lane; i < CS * (dim() / 8); i += 32) {
+                const int64_t j = t0 + i / (dim() / 8);
+                if (!((j < v.first || j >= v.begin) && j < v.len))
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(stage + CS * rb + i * 16u), "r"(0u) : "memory");
+            }
+            /* the stage's next rows come through the other proxy */
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
         }
         float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < CS / 8; i++) {
-            if (!WHOLE) {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (!((vis >> (2 * i + (e & 1))) & 1u)) s[i][e] = -INFINITY;
-            }
             mx0 = fmaxf(mx0, fmaxf(s[i][0], s[i][1]));
             mx1 = fmaxf(mx1, fmaxf(s[i][2], s[i][3]));
         }
@@ -453,50 +481,41 @@ struct KvAttendWork {
         const float c0 = n0 == -INFINITY ? 0.f : n0, c1 = n1 == -INFINITY ? 0.f : n1;     /* nothing seen yet: exp2(-inf - 0) = 0 */
         if (__any_sync(0xffffffffu, n0 != z.m[0] || n1 != z.m[1])) {
             const float a0 = exp2_fast(z.m[0] - c0), a1 = exp2_fast(z.m[1] - c1);
+            float a[NT][2];
+            to_columns(a0, a1, a);
             z.l[0] *= a0; z.l[1] *= a1;
 #pragma unroll
-            for (int i = 0; i < DMAX / 8; i++) { z.o[i][0] *= a0; z.o[i][1] *= a0; z.o[i][2] *= a1; z.o[i][3] *= a1; }
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < DMAX / 16; i++) { z.o[n][i][0] *= a[n][0]; z.o[n][i][1] *= a[n][1]; z.o[n][i][2] *= a[n][0]; z.o[n][i][3] *= a[n][1]; }
             z.m[0] = n0; z.m[1] = n1;
         }
-        const uint32_t v_row = stage + CS * rb + ((lane & 7u) + ((lane >> 3) & 1u) * 8u) * rb, v_c = (lane >> 4) & 1u;
-        uint32_t hi[CS / 16][4], lo[CS / 16][4];
+        const uint32_t v_row = stage + CS * rb + ((lane & 7u) + ((lane >> 4) & 1u) * 8u) * rb, v_c = (lane >> 3) & 1u;
+        uint32_t hi[NT][CS / 8], lo[NT][CS / 8];
 #pragma unroll
         for (int i = 0; i < CS / 8; i++) {
-            float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                p[e] = exp2_fast(fmaf(s[i][e], scale_log2, e < 2 ? -c0 : -c1));
-                if (!WHOLE && !((vis >> (2 * i + (e & 1))) & 1u)) p[e] = 0.f;
+            for (int n = 0; n < NT; n++) {
+                float p[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) p[e] = exp2_fast(fmaf(s[i][2 * n + e], scale_log2, n ? -c1 : -c0));
+                z.l[n] += p[0] + p[1];
+                hi[n][i] = kv_type<T>::pack(p[0], p[1]);
+                const float2 h = kv_type<T>::unpack(hi[n][i]);
+                lo[n][i] = kv_type<T>::pack(p[0] - h.x, p[1] - h.y);
             }
-            z.l[0] += p[0] + p[1];
-            z.l[1] += p[2] + p[3];
-            uint32_t* h = hi[i / 2] + 2 * (i & 1);
-            uint32_t* l = lo[i / 2] + 2 * (i & 1);
-            h[0] = kv_type<T>::pack(p[0], p[1]);
-            h[1] = kv_type<T>::pack(p[2], p[3]);
-            const float2 h0 = kv_type<T>::unpack(h[0]), h1 = kv_type<T>::unpack(h[1]);
-            l[0] = kv_type<T>::pack(p[0] - h0.x, p[1] - h0.y);
-            l[1] = kv_type<T>::pack(p[2] - h1.x, p[3] - h1.y);
         }
 #pragma unroll
         for (int kt = 0; kt < CS / 16; kt++) {
-            /* rows that are not visible may hold anything, and 0 x NaN is not 0: they become zeros */
-            uint32_t k0 = 0, k1 = 0;
-            if (!WHOLE) {
-                const uint32_t bits = vis >> (4 * kt);
-                k0 = ((bits & 1u) ? 0x0000ffffu : 0u) | ((bits & 2u) ? 0xffff0000u : 0u);
-                k1 = ((bits & 4u) ? 0x0000ffffu : 0u) | ((bits & 8u) ? 0xffff0000u : 0u);
-            }
 #pragma unroll
-            for (int np = 0; np < DMAX / 16; np++) {
-                if (EXACT || np * 16 < (int)L.head_dim) {
+            for (int mt = 0; mt < DMAX / 16; mt++) {
+                if (EXACT || mt * 16 < (int)L.head_dim) {
                     uint32_t r[4];
-                    ldm_x4_t(r, at(v_row, v_c, np * 2) + kt * 16 * rb);
-                    if (!WHOLE) { r[0] &= k0; r[1] &= k1; r[2] &= k0; r[3] &= k1; }
-                    mma_16816(z.o[2 * np], hi[kt], r[0], r[1], T());
-                    mma_16816(z.o[2 * np + 1], hi[kt], r[2], r[3], T());
-                    mma_16816(z.o[2 * np], lo[kt], r[0], r[1], T());
-                    mma_16816(z.o[2 * np + 1], lo[kt], r[2], r[3], T());
+                    ldm_x4_t(r, at(v_row, v_c, mt * 2) + kt * 16 * rb);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma_16816(z.o[n][mt], r, hi[n][2 * kt], hi[n][2 * kt + 1], T());
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma_16816(z.o[n][mt], r, lo[n][2 * kt], lo[n][2 * kt + 1], T());
                 }
             }
         }
@@ -514,18 +533,31 @@ struct KvAttendWork {
     BAM_DEV void write_out(const state_t& z, uint32_t b, uint32_t u) const
     {
         const uint32_t lane = lane_id(), h = u / tiles, r0 = (u - h * tiles) * KV_ROWS;
+        float inv[NT][2];
+        to_columns(z.l[0] == 0.f ? 0.f : 1.f / z.l[0], z.l[1] == 0.f ? 0.f : 1.f / z.l[1], inv);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint32_t r = r0 + 8 * n + (lane & 3u) * 2 + e;
+                uint16_t* p = out + b * o_sb + (h * group + r) * o_sh;
+#pragma unroll
+                for (int i = 0; i < DMAX / 16; i++) {
+                    if (EXACT || i * 16 < (int)L.head_dim) {
+                        /* neighbours in a row of the output sit four lanes apart: the even row of threads takes a pair from
+                         * the dimensions r, the odd one from r + 8 */
+                        const float a = z.o[n][i][e] * inv[n][e], c = z.o[n][i][2 + e] * inv[n][e];
+                        const bool odd = lane & 4u;
+                        const float other = __shfl_xor_sync(0xffffffffu, odd ? a : c, 4);
+                        if (r < group) store_pair(p + i * 16 + (odd ? 8 : 0) + ((lane >> 2) & 6u), odd ? other : a, odd ? c : other);
+                    }
+                }
+            }
+        }
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const uint32_t r = r0 + (lane >> 2) + 8 * half;
-            if (r < group) {
-                const uint32_t hq = h * group + r;
-                const float inv = z.l[half] == 0.f ? 0.f : 1.f / z.l[half];
-                uint16_t* p = out + b * o_sb + hq * o_sh + (lane & 3u) * 2;
-#pragma unroll
-                for (int i = 0; i < DMAX / 8; i++)
-                    if (i * 8 < (int)L.head_dim || EXACT) store_pair(p + i * 8, z.o[i][2 * half] * inv, z.o[i][2 * half + 1] * inv);
-                if (lse && (lane & 3u) == 0u) lse[(size_t)b * n_q_heads + hq] = lse_of(z.m[half], z.l[half]);
-            }
+            if (lse && (lane & 3u) == 0u && r < group) lse[(size_t)b * n_q_heads + h * group + r] = lse_of(z.m[half], z.l[half]);
         }
     }
     /* query heads of unit u */
@@ -534,24 +566,28 @@ struct KvAttendWork {
         const uint32_t r0 = u % tiles * KV_ROWS;
         return group - r0 < KV_ROWS ? group - r0 : KV_ROWS;
     }
+    /* A part of a unit in the scratch: maxima and denominators by query, and the sums as the registers hold them, quad
+     * [n][i][lane]: dimensions 16 i + lane / 4 and + 8 of queries 8 n + 2 (lane % 4) and + 1. */
     BAM_DEV void write_part(const state_t& z, float* p, uint32_t rows) const
     {
         const uint32_t lane = lane_id();
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const uint32_t r = (lane >> 2) + 8 * half;
-            if (r < rows) {
-                float* row = p + r * dim() + (lane & 3u) * 2;
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int i = 0; i < DMAX / 8; i++)
-                    if (EXACT || i * 8 < (int)L.head_dim) st_cg_f2(row + i * 8, z.o[i][2 * half], z.o[i][2 * half + 1]);
-                if ((lane & 3u) == 0u) st_cg_f2(p + KV_ROWS * dim() + 2 * r, z.m[half], z.l[half]);
-            }
+            for (int i = 0; i < DMAX / 16; i++)
+                if ((EXACT || i * 16 < (int)L.head_dim) && 8 * n + (lane & 3u) * 2 < rows) {
+                    float* q_ = p + ((n * (dim() / 16) + i) * 32 + lane) * 4;
+                    st_cg_f4(q_, z.o[n][i][0], z.o[n][i][1], z.o[n][i][2], z.o[n][i][3]);
+                }
+        if ((lane & 3u) == 0u) {
+            float* ml = p + KV_ROWS * dim() + 2 * (lane >> 2);
+            st_cg_f2(ml, z.m[0], z.l[0]);
+            st_cg_f2(ml + 16, z.m[1], z.l[1]);
         }
     }
 
     /* ---- a worker ------------------------------------------------------------------------------------- */
-    BAM_DEV void work(kv_shared_t& sh, uint32_t ring, uint64_t per, uint32_t worker) const
+    BAM_DEV void work(kv_shared_t& sh, uint32_t ring, const list_t& list, uint32_t worker) const
     {
         const uint32_t lane = lane_id(), w = threadIdx.x >> 5, units = L.n_kv_heads * tiles;
         pipe_t g;
@@ -576,7 +612,7 @@ struct KvAttendWork {
             const uint16_t* q1 = r0 + 8 < group ? q + b * q_sb + (int64_t)(h * group + r0 + 8) * q_sh : nullptr;
             state_t z;
 #pragma unroll
-            for (int i = 0; i < DMAX / 8; i++) z.o[i][0] = z.o[i][1] = z.o[i][2] = z.o[i][3] = 0.f;
+            for (int i = 0; i < NT * (DMAX / 16); i++) { float* o = z.o[i / (DMAX / 16)][i % (DMAX / 16)]; o[0] = o[1] = o[2] = o[3] = 0.f; }
             z.m[0] = z.m[1] = -INFINITY;
             z.l[0] = z.l[1] = 0.f;
             uint32_t qa[DMAX / 16][4];
@@ -585,9 +621,7 @@ struct KvAttendWork {
                 if (!landed(sh, g)) break;
                 unpin(sh, g);
                 const uint32_t stage = g.base + g.stage * stage_bytes();
-                const int64_t t0 = first_token(v, c + i);
-                if (t0 + CS <= v.first || (t0 >= v.begin && t0 + CS <= v.len)) chunk<true>(z, qa, stage, v, t0);
-                else chunk<false>(z, qa, stage, v, t0);
+                chunk(z, qa, stage, v, first_token(v, c + i));
                 __syncwarp();
                 advance(g);
             }
@@ -601,12 +635,12 @@ struct KvAttendWork {
             else {
                 const uint64_t U0 = f - c;
                 uint32_t i0, cnt;
-                workers_of(U0, U0 + v.n, per, i0, cnt);
+                workers_of(U0, U0 + v.n, list, i0, cnt);
                 write_part(z, part(worker, worker == i0 ? 1 : 0), rows_of(u));
-                __threadfence();
                 __syncwarp();
                 if (lane == 0) {
-                    (void)atom_add_acq_rel(arrived + i0, 1u);
+                    /* one release for the warp: what its other lanes wrote comes before it by the barrier */
+                    red_add_release(arrived + i0, 1u);
                     sh.join[w][n_join].b = b; sh.join[w][n_join].u = u; sh.join[w][n_join].first = U0; sh.join[w][n_join].n = v.n;
                 }
                 n_join++;
@@ -627,15 +661,15 @@ struct KvAttendWork {
             return;
         }
         __syncwarp();
-        for (uint32_t k = 0; k < n_join; k++) join(sh, sh.join[w][k].b, sh.join[w][k].u, sh.join[w][k].first, sh.join[w][k].n, per, worker);
+        for (uint32_t k = 0; k < n_join; k++) join(sh, sh.join[w][k].b, sh.join[w][k].u, sh.join[w][k].first, sh.join[w][k].n, list, worker);
     }
 
     /* This worker's share of a unit that several worked on. */
-    BAM_DEV void join(kv_shared_t& sh, uint32_t b, uint32_t u, uint64_t U0, uint32_t n, uint64_t per, uint32_t worker) const
+    BAM_DEV void join(kv_shared_t& sh, uint32_t b, uint32_t u, uint64_t U0, uint32_t n, const list_t& list, uint32_t worker) const
     {
         const uint32_t lane = lane_id(), D = dim();
         uint32_t i0, cnt;
-        workers_of(U0, U0 + n, per, i0, cnt);
+        workers_of(U0, U0 + n, list, i0, cnt);
         bam_status_t* st = L.r.cache.status;
         uint32_t polls = 0, gone = 0;
         uint64_t t0 = 0;
@@ -651,83 +685,99 @@ struct KvAttendWork {
         }
         if (__shfl_sync(0xffffffffu, gone, 0)) return;
         const uint32_t h = u / tiles, r0 = (u - h * tiles) * KV_ROWS;
-        const uint32_t quads = rows_of(u) * (D / 4), j = worker - i0;
+        const uint32_t rows = rows_of(u), quads = (rows + 7) / 8 * (D / 16) * 32, j = worker - i0;
         const uint32_t g0 = (uint32_t)((uint64_t)quads * j / cnt), g1 = (uint32_t)((uint64_t)quads * (j + 1) / cnt);
-        /* A quad is four elements of the output; P lanes share one, each adds up to eight parts at a time.  Two quads of a
-         * lane are loaded together, and all loads are issued before the first is used: a part is one access to L2, and
-         * one after the other they took 10 to 15 us of a call. */
+        /* A quad is four elements of the output (see write_part); P lanes share one, each adds up to four parts of two quads
+         * at a time, whose loads are all issued before the first is used: a part is one access to L2, and one after the
+         * other they took 10 to 15 us of a call. */
         uint32_t P = 1;
-        while (P * 8 < cnt && P < 32u) P <<= 1;
+        while (P * 4 < cnt && P < 32u) P <<= 1;
         const uint32_t p = lane & (P - 1u), at_once = 32u / P;
+#pragma unroll 1
         for (uint32_t base = g0; base < g1; base += 2 * at_once) {
-            float M[2], l[2], x[2][4];
-            uint32_t r[2], d[2];
+            /* of two queries, q0 and q0 + 1 */
+            uint32_t gi[2], q0[2];
             bool act[2];
+            float M[2][2], l[2][2], x[2][4];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const uint32_t gi = base + e * at_once + lane / P;
-                act[e] = gi < g1;
-                r[e] = act[e] ? gi / (D / 4) : 0;
-                d[e] = act[e] ? (gi - r[e] * (D / 4)) * 4 : 0;
-                M[e] = -INFINITY; l[e] = 0.f;
-                x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.f;
+                gi[e] = base + e * at_once + lane / P;
+                q0[e] = gi[e] / (32u * (D / 16)) * 8 + (gi[e] & 3u) * 2;
+                act[e] = gi[e] < g1 && q0[e] < rows;
+                M[e][0] = M[e][1] = -INFINITY;
+                l[e][0] = l[e][1] = x[e][0] = x[e][1] = x[e][2] = x[e][3] = 0.f;
             }
-            for (uint32_t s0 = 0; s0 < cnt; s0 += 8 * P) {
-                float2 ml[2][8];
-                uint4 y[2][8];
+#pragma unroll 1
+            for (uint32_t s0 = 0; s0 < cnt; s0 += 4 * P) {
+                uint4 ml[2][4], y[2][4];
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
+                for (int k = 0; k < 4; k++) {
                     const uint32_t s = s0 + k * P + p;
+                    const float* y_ = part(i0 + s, s == 0 ? 1 : 0);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        ml[e][k] = make_float2(-INFINITY, 0.f);
+                        ml[e][k] = make_uint4(0xff800000u, 0u, 0xff800000u, 0u);              /* -infinity, 0 */
                         y[e][k] = make_uint4(0, 0, 0, 0);
                         if (s < cnt && act[e]) {
-                            const float* y_ = part(i0 + s, s == 0 ? 1 : 0);
-                            ml[e][k] = ld_cg_f2(y_ + KV_ROWS * D + 2 * r[e]);
-                            y[e][k] = ld_cg_v4(y_ + r[e] * D + d[e]);
+                            ml[e][k] = ld_cg_v4(y_ + KV_ROWS * D + 2 * q0[e]);
+                            y[e][k] = ld_cg_v4(y_ + (size_t)gi[e] * 4);
                         }
                     }
                 }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float m = M[e];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) m = fmaxf(m, ml[e][k].x);
-                    const float c = m == -INFINITY ? 0.f : m, a = exp2_fast(M[e] - c);
-                    M[e] = m;
-                    l[e] *= a;
+                    for (int c2 = 0; c2 < 2; c2++) {
+                        float m = M[e][c2];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x[e][i] *= a;
+                        for (int k = 0; k < 4; k++) m = fmaxf(m, __uint_as_float(c2 ? ml[e][k].z : ml[e][k].x));
+                        const float c = m == -INFINITY ? 0.f : m, a = exp2_fast(M[e][c2] - c);
+                        M[e][c2] = m;
+                        l[e][c2] *= a; x[e][c2] *= a; x[e][2 + c2] *= a;
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const float a1 = exp2_fast(ml[e][k].x - c);
-                        l[e] += ml[e][k].y * a1;
-                        x[e][0] += __uint_as_float(y[e][k].x) * a1; x[e][1] += __uint_as_float(y[e][k].y) * a1;
-                        x[e][2] += __uint_as_float(y[e][k].z) * a1; x[e][3] += __uint_as_float(y[e][k].w) * a1;
+                        for (int k = 0; k < 4; k++) {
+                            const float a1 = exp2_fast(__uint_as_float(c2 ? ml[e][k].z : ml[e][k].x) - c);
+                            l[e][c2] += __uint_as_float(c2 ? ml[e][k].w : ml[e][k].y) * a1;
+                            x[e][c2] += __uint_as_float(c2 ? y[e][k].y : y[e][k].x) * a1;
+                            x[e][2 + c2] += __uint_as_float(c2 ? y[e][k].w : y[e][k].z) * a1;
+                        }
                     }
                 }
             }
+            float all[2][2] = { { M[0][0], M[0][1] }, { M[1][0], M[1][1] } };
+#pragma unroll 1
+            for (uint32_t o = P >> 1; o > 0; o >>= 1) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float all = M[e];
-                for (uint32_t o = P >> 1; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-                const float a = exp2_fast(M[e] - (all == -INFINITY ? 0.f : all));
-                l[e] *= a;
+                for (int i = 0; i < 4; i++) all[i >> 1][i & 1] = fmaxf(all[i >> 1][i & 1], __shfl_xor_sync(0xffffffffu, all[i >> 1][i & 1], o));
+            }
 #pragma unroll
-                for (int i = 0; i < 4; i++) x[e][i] *= a;
-                for (uint32_t o = P >> 1; o > 0; o >>= 1) {
-                    l[e] += __shfl_xor_sync(0xffffffffu, l[e], o);
+            for (int i = 0; i < 4; i++) {
+                const float a = exp2_fast(M[i >> 1][i & 1] - (all[i >> 1][i & 1] == -INFINITY ? 0.f : all[i >> 1][i & 1]));
+                l[i >> 1][i & 1] *= a; x[i >> 1][i & 1] *= a; x[i >> 1][2 + (i & 1)] *= a;
+            }
+#pragma unroll 1
+            for (uint32_t o = P >> 1; o > 0; o >>= 1) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) x[e][i] += __shfl_xor_sync(0xffffffffu, x[e][i], o);
+                    l[e][0] += __shfl_xor_sync(0xffffffffu, l[e][0], o);
+                    l[e][1] += __shfl_xor_sync(0xffffffffu, l[e][1], o);
                 }
-                if (act[e] && p == 0) {
-                    const uint32_t hq = h * group + r0 + r[e];
-                    const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
-                    uint16_t* dst = out + b * o_sb + hq * o_sh + d[e];
-                    store_pair(dst, x[e][0] * inv, x[e][1] * inv);
-                    store_pair(dst + 2, x[e][2] * inv, x[e][3] * inv);
-                    if (lse && d[e] == 0) lse[(size_t)b * n_q_heads + hq] = lse_of(all, l[e]);
+            }
+            if (p == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = i >> 1, c2 = i & 1;
+                    if (act[e] && q0[e] + c2 < rows) {
+                        const uint32_t hq = h * group + r0 + q0[e] + c2, d = gi[e] / 32 % (D / 16) * 16 + (gi[e] >> 2) % 8;
+                        const float inv = l[e][c2] == 0.f ? 0.f : 1.f / l[e][c2];
+                        uint16_t* dst = out + b * o_sb + hq * o_sh + d;
+                        const uint32_t w = kv_type<T>::pack(x[e][c2] * inv, x[e][2 + c2] * inv);
+                        dst[0] = (uint16_t)w;
+                        dst[8] = (uint16_t)(w >> 16);
+                        if (lse && d == 0) lse[(size_t)b * n_q_heads + hq] = lse_of(all[e][c2], l[e][c2]);
+                    }
                 }
             }
         }
@@ -775,10 +825,11 @@ struct KvAttendWork {
         }
         total *= units;
         sh.before[t] = before * units;
-        const uint64_t n_workers = (uint64_t)nvb * KV_WORKERS;
-        uint64_t per = (total + n_workers - 1) / n_workers;
-        const uint32_t least = longest < KV_MIN_CHUNKS ? longest : KV_MIN_CHUNKS;
-        if (per < least) per = least;
+        /* workers: all there are, but none of them with less than KV_MIN_CHUNKS (or the longest unit, if that is shorter) */
+        const uint64_t n_workers = (uint64_t)nvb * KV_WORKERS, least = longest < KV_MIN_CHUNKS ? longest : KV_MIN_CHUNKS;
+        list_t list = { total, total >= n_workers * least ? n_workers : total / (least ? least : 1u), 0 };
+        if (list.workers == 0) list.workers = 1;
+        list.slack = total / list.workers / 8 < 2 ? total / list.workers / 8 : 2;
         /* sequences with nothing visible */
         for (uint32_t b = vb; b < batch; b += nvb) {
             if (seen(b).n == 0) {
@@ -793,12 +844,14 @@ struct KvAttendWork {
         /* neighbours in the list on different SMs: the workers of a short list spread out */
         const uint32_t worker = w * nvb + vb;
         if (w < KV_WORKERS) {
-            const kv_place_t from = cut(sh, worker, per, total), to = cut(sh, worker + 1ull, per, total);
+            kv_place_t from = { 0, 0, 0 }, to = from;
+#pragma unroll 1
+            for (uint32_t k = 0; k < 2; k++) { from = to; to = begin_of(sh, worker + (uint64_t)k, list); }
             if (lane == 0) { sh.from[w] = from; sh.chunks[w] = (uint32_t)(to.f - from.f); }
         }
         __syncthreads();
         if (w < KV_WORKERS) {
-            if (sh.chunks[w]) work(sh, ring, per, worker);
+            if (sh.chunks[w]) work(sh, ring, list, worker);
         } else pin_ahead(sh, vb);
         __syncthreads();
         if (sh.abort && t < KV_WORKERS * KV_AHEAD && (sh.tag[0][t] & 1u)) {            /* given up: what was pinned and never copied */
@@ -808,10 +861,10 @@ struct KvAttendWork {
     }
 };
 
-template <class T, int DMAX, int CS, bool EXACT>
-static int launch_attend_as(bam_array* a, const kv_layout_d_t& L, const bam_kv_attend_t* p, void* scratch, void* stream)
+template <class T, int DMAX, int CS, bool EXACT, int NT>
+static int launch_attend_nt(bam_array* a, const kv_layout_d_t& L, const bam_kv_attend_t* p, void* scratch, void* stream)
 {
-    typedef KvAttendWork<T, DMAX, CS, EXACT> Work;
+    typedef KvAttendWork<T, DMAX, CS, EXACT, NT> Work;
     Work w;
     memset(&w, 0, sizeof w);
     w.L = L;
@@ -820,7 +873,8 @@ static int launch_attend_as(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     w.table = p->block_table; w.table_stride = p->table_stride; w.table_width = p->table_width; w.lens = p->seq_lens;
     w.batch = p->batch; w.n_q_heads = p->n_q_heads;
     w.group = p->n_q_heads / L.n_kv_heads; w.tiles = (w.group + KV_ROWS - 1) / KV_ROWS;
-    w.scale_log2 = fabsf(p->scale) * 1.4426950408889634f;
+    /* never 0: -infinity x 0, of a score that is not visible, would be NaN */
+    w.scale_log2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, 1e-30f);
     w.q_sign = p->scale < 0.f ? 0x80008000u : 0u;
     w.window = p->window; w.sinks = p->sinks;
     w.q32 = ((uintptr_t)p->q & 3) == 0 && p->q_stride[0] % 2 == 0 && p->q_stride[1] % 2 == 0;
@@ -830,9 +884,6 @@ static int launch_attend_as(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     w.arrived = (uint32_t*)(base + sizeof(kv_launch_words_t));
     w.parts = (float*)(base + kv_parts_at(most * KV_WORKERS));
     w.piece = L.block_tokens % CS == 0 ? CS : 16;
-    /* what all workers may hold pinned is at most half of the cache (one chunk each where that is too little) */
-    const uint64_t share = a->pc->d.n_slots / 2 / ((uint64_t)most * KV_WORKERS * (CS / w.piece));
-    w.ahead = share < 1 ? 1u : share < KV_AHEAD ? (uint32_t)share : KV_AHEAD;
     /* no more blocks than the longest sequences could keep busy */
     uint64_t chunks = ((uint64_t)p->table_width * L.block_tokens + CS - 1) / CS;
     if (p->window > 0) {
@@ -842,7 +893,19 @@ static int launch_attend_as(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     const uint32_t least = chunks < KV_MIN_CHUNKS ? (uint32_t)chunks : KV_MIN_CHUNKS;
     const uint64_t workers = (chunks * p->batch * L.n_kv_heads * w.tiles + least - 1) / least;
     const uint64_t want = (workers + KV_WORKERS - 1) / KV_WORKERS;
-    return kv_launch(a->pc->ctrl, w, want < most ? want : most, scratch, sizeof(kv_launch_words_t) + 4 * (size_t)most * KV_WORKERS, (cudaStream_t)stream);
+    const uint64_t blocks = want < most ? want : most;
+    /* no more pinned than the cache has slots; two chunks all the same, or copies would not overlap (a cache that is too
+     * full for that makes the pinning warps ask for less) */
+    const uint64_t share = a->pc->d.n_slots / (blocks * KV_WORKERS * (CS / w.piece));
+    w.ahead = share < 2 ? 2u : share < KV_AHEAD ? (uint32_t)share : KV_AHEAD;
+    return kv_launch(a->pc->ctrl, w, blocks, scratch, sizeof(kv_launch_words_t) + 4 * (size_t)most * KV_WORKERS, (cudaStream_t)stream);
+}
+
+template <class T, int DMAX, int CS, bool EXACT>
+static int launch_attend_as(bam_array* a, const kv_layout_d_t& L, const bam_kv_attend_t* p, void* scratch, void* stream)
+{
+    return p->n_q_heads / L.n_kv_heads <= 8 ? launch_attend_nt<T, DMAX, CS, EXACT, 1>(a, L, p, scratch, stream)
+                                            : launch_attend_nt<T, DMAX, CS, EXACT, 2>(a, L, p, scratch, stream);
 }
 
 template <class T>

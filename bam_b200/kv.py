@@ -41,9 +41,9 @@ class KvCache:
         self.block_tokens, self.n_layers = block_tokens, n_layers
         self.device = torch.device("cuda", cache.ctrl.device)
         self.array = Array(cache, n_layers * n_blocks * n_kv_heads * (cache.page_size // 8), 8, store_byte_offset, dist)
-        self._layouts = [KvLayout(0 if dtype == torch.bfloat16 else 1, head_dim, n_kv_heads, block_tokens, n_blocks,
-                                  i * n_blocks * n_kv_heads) for i in range(n_layers)]
-        self._scratch_bytes = self.lib.bam_kv_scratch_bytes(self.array.h, C.byref(self._layouts[0]))
+        self._layouts = [C.byref(KvLayout(0 if dtype == torch.bfloat16 else 1, head_dim, n_kv_heads, block_tokens, n_blocks,
+                                          i * n_blocks * n_kv_heads)) for i in range(n_layers)]
+        self._scratch_bytes = self.lib.bam_kv_scratch_bytes(self.array.h, self._layouts[0])
 
     def close(self):
         self.array.close()
@@ -53,56 +53,50 @@ class KvCache:
     def _layout(self, layer):
         if not 0 <= layer < self.n_layers:
             raise ValueError(f"layer {layer} of {self.n_layers}")
-        return C.byref(self._layouts[layer])
+        return self._layouts[layer]
 
     def _on(self, name, t, dtype, ndim):
+        if t.dtype is dtype and t.dim() == ndim and t.device == self.device:
+            return t
         if t.device != self.device:
             raise ValueError(f"{name} is on {t.device}, the cache on {self.device}")
         if t.dtype != dtype:
             raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-        if t.dim() != ndim:
-            raise ValueError(f"{name} must have {ndim} dimensions, not {t.dim()}")
-        return t
+        raise ValueError(f"{name} must have {ndim} dimensions, not {t.dim()}")
 
     def _heads(self, name, t, n, heads):
-        """A tensor [n, heads, head_dim] whose heads are contiguous."""
+        """The strides of a tensor [n, heads, head_dim] whose heads are contiguous."""
         self._on(name, t, self.dtype, 3)
-        if (n is not None and t.shape[0] != n) or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, wanted ({'n' if n is None else n}, {heads}, {self.head_dim})")
-        if t.stride(2) != 1:
+        shape, stride = t.shape, t.stride()
+        if (n is not None and shape[0] != n) or shape[1] != heads or shape[2] != self.head_dim:
+            raise ValueError(f"{name} has shape {tuple(shape)}, wanted ({'n' if n is None else n}, {heads}, {self.head_dim})")
+        if stride[2] != 1:
             raise ValueError(f"the elements of a head of {name} must be contiguous")
-        return t
+        return stride[:2]
 
     def _flat(self, name, t, dtype, n):
+        """The address of n contiguous values."""
         self._on(name, t, dtype, 1)
         if t.shape[0] != n or (n > 1 and t.stride(0) != 1):
             raise ValueError(f"{name} must be {n} contiguous values")
-        return t
+        return t.data_ptr()
 
-    def _queue(self, stream):
-        """The stream the call runs on, as a context for the memory it takes: `stream` (a torch stream or a raw
-        handle), or torch's current stream of the cache's device."""
+    def _on_stream(self, stream):
+        """`stream` (a torch stream or a raw handle) as the context the call takes its memory and runs in."""
         import torch
-        if stream is None:
-            return None
         if not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(int(stream), device=self.device)
         if stream.device != self.device:
             raise ValueError(f"the stream is on {stream.device}, the cache on {self.device}")
-        return stream
+        return torch.cuda.stream(stream)
 
-    def _run(self, stream, call):
+    def _call(self, name, layer, *args):
+        """A launch on the current stream of the cache's device, with scratch memory of its own (so that calls on other
+        streams and captured ones, whose scratch belongs to their graph, do not meet in it)."""
         import torch
-        s = self._queue(stream)
-        if s is None:
-            s = torch.cuda.current_stream(self.device)
-            return call(s.cuda_stream)
-        with torch.cuda.stream(s):
-            return call(s.cuda_stream)
-
-    def _scratch(self):
-        import torch
-        return torch.empty(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        check(getattr(self.lib, name)(self.array.h, layer, *args, scratch.data_ptr(), self._scratch_bytes,
+                                      torch.cuda.current_stream(self.device.index).cuda_stream), name)
 
     # ---- operators ----------------------------------------------------------------------------------------
 
@@ -118,12 +112,15 @@ class KvCache:
         ("pairs").  `q` ([n, heads, head_dim]) takes the same pass with `q_norm`, into `q_out` (may be q itself) or a
         new tensor, which is returned.  All of it is computed in 32 bits and rounded once."""
         import torch
+        if stream is not None:
+            with self._on_stream(stream):
+                return self.append(k, v, slots, layer, positions, rope, rope_style, q, q_norm, k_norm, norm_eps, q_out)
         n = k.shape[0]
-        self._heads("k", k, None, self.n_kv_heads)
-        self._heads("v", v, n, self.n_kv_heads)
-        self._flat("slots", slots, torch.int64, n)
-        a = KvAppend(k=k.data_ptr(), v=v.data_ptr(), n_tokens=n, slots=slots.data_ptr(), norm_eps=norm_eps)
-        a.k_stride[:], a.v_stride[:] = k.stride()[:2], v.stride()[:2]
+        a = KvAppend()
+        a.k_stride = self._heads("k", k, None, self.n_kv_heads)
+        a.v_stride = self._heads("v", v, n, self.n_kv_heads)
+        a.slots = self._flat("slots", slots, torch.int64, n)
+        a.k, a.v, a.n_tokens, a.norm_eps = k.data_ptr(), v.data_ptr(), n, norm_eps
         if rope is not None:
             cos, sin = rope
             self._on("cos", cos, torch.float32, 2)
@@ -132,64 +129,55 @@ class KvCache:
                 raise ValueError(f"rope_style must be one of {sorted(ROPE_STYLES)}, not {rope_style!r}")
             if positions is None:
                 raise ValueError("a rotation needs positions")
-            self._flat("positions", positions, torch.int64, n)
-            if cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1 or cos.shape[0] == 0:
+            a.positions = self._flat("positions", positions, torch.int64, n)
+            (rows, half), stride = cos.shape, cos.stride()
+            if sin.shape != cos.shape or sin.stride() != stride or stride[1] != 1 or rows == 0:
                 raise ValueError("cos and sin must be rows of the same shape and strides")
-            rotary = 2 * cos.shape[1]
+            rotary = 2 * half
             if rotary % 16 or not 0 < rotary <= self.head_dim:
                 raise ValueError(f"{rotary} rotated elements: a multiple of 16 up to {self.head_dim} is wanted")
-            a.positions, a.cos, a.sin, a.n_positions = positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-            a.rope_stride, a.rotary_dim, a.rope_style = max(cos.stride(0), rotary // 2), rotary, ROPE_STYLES[rope_style]
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None:
-                setattr(a, name, self._flat(name, w, self.dtype, self.head_dim).data_ptr())
+            a.cos, a.sin, a.n_positions = cos.data_ptr(), sin.data_ptr(), rows
+            a.rope_stride, a.rotary_dim, a.rope_style = max(stride[0], half), rotary, ROPE_STYLES[rope_style]
+        if q_norm is not None:
+            a.q_norm = self._flat("q_norm", q_norm, self.dtype, self.head_dim)
+        if k_norm is not None:
+            a.k_norm = self._flat("k_norm", k_norm, self.dtype, self.head_dim)
+        layout = self._layout(layer)
         if q is None:
             if q_norm is not None or q_out is not None:
                 raise ValueError("q_norm and q_out go with q")
         else:
             if q.dim() != 3 or q.shape[1] < 1:
                 raise ValueError("q must be [n, heads, head_dim]")
-            self._heads("q", q, n, q.shape[1])
-            if q_out is not None:
-                self._heads("q_out", q_out, n, q.shape[1])
-
-        def call(s):
-            out = q_out
-            if q is not None:
-                if out is None:
-                    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-                a.q, a.q_out, a.n_q_heads = q.data_ptr(), out.data_ptr(), q.shape[1]
-                a.q_stride[:], a.q_out_stride[:] = q.stride()[:2], out.stride()[:2]
-            scratch = self._scratch()
-            check(self.lib.bam_launch_kv_append(self.array.h, self._layout(layer), C.byref(a), scratch.data_ptr(),
-                                                self._scratch_bytes, s), "bam_launch_kv_append")
-            return out
-        if n == 0:
-            self._layout(layer)
-            return q_out if q is None or q_out is not None else torch.empty_like(q)
-        return self._run(stream, call)
+            a.n_q_heads = q.shape[1]
+            a.q_stride = self._heads("q", q, n, a.n_q_heads)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
+            a.q_out_stride = self._heads("q_out", q_out, n, a.n_q_heads)
+            a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+        if n:
+            self._call("bam_launch_kv_append", layout, C.byref(a))
+        return q_out
 
     def gather(self, slots, layer=0, out=None, stream=None):
         """The rows at `slots` (int64; negative: zeros) as (k, v), each [n, n_kv_heads, head_dim]; `out`: a pair of
         tensors of that shape, with any strides of tokens and heads, to write them to."""
         import torch
+        if stream is not None:
+            with self._on_stream(stream):
+                return self.gather(slots, layer, out)
         n = slots.shape[0] if slots.dim() == 1 else -1
-        self._flat("slots", slots, torch.int64, n)
-        if out is not None:
-            self._heads("out[0]", out[0], n, self.n_kv_heads)
-            self._heads("out[1]", out[1], n, self.n_kv_heads)
-
-        def call(s):
-            k, v = out if out is not None else (torch.empty((n, self.n_kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
-                                                for _ in range(2))
-            ks, vs = (C.c_int64 * 2)(*k.stride()[:2]), (C.c_int64 * 2)(*v.stride()[:2])
-            scratch = self._scratch()
-            if n:
-                check(self.lib.bam_launch_kv_gather(self.array.h, self._layout(layer), n, slots.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                                    ks, vs, scratch.data_ptr(), self._scratch_bytes, s), "bam_launch_kv_gather")
-            return k, v
-        self._layout(layer)
-        return self._run(stream, call)
+        at = self._flat("slots", slots, torch.int64, n)
+        layout = self._layout(layer)
+        if out is None:
+            shape = (n, self.n_kv_heads, self.head_dim)
+            out = (torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device))
+        k, v = out
+        ks = (C.c_int64 * 2)(*self._heads("out[0]", k, n, self.n_kv_heads))
+        vs = (C.c_int64 * 2)(*self._heads("out[1]", v, n, self.n_kv_heads))
+        if n:
+            self._call("bam_launch_kv_gather", layout, n, at, k.data_ptr(), v.data_ptr(), ks, vs)
+        return k, v
 
     def attend(self, q, block_table, seq_lens, layer=0, scale=None, window=0, sinks=0, out=None, return_lse=False, stream=None):
         """Attention of one new token per sequence: q [batch, heads, head_dim] (heads a multiple of n_kv_heads) over the
@@ -200,31 +188,32 @@ class KvCache:
         (out, lse) with the logarithm of the softmax's denominator [batch, heads]; a sequence with nothing visible gets
         zeros and -inf.  The new token's own key and value have to be appended first."""
         import torch
+        if stream is not None:
+            with self._on_stream(stream):
+                return self.attend(q, block_table, seq_lens, layer, scale, window, sinks, out, return_lse)
         if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.n_kv_heads:
             raise ValueError(f"q must be [batch, heads, head_dim] with a multiple of {self.n_kv_heads} heads")
-        n, heads = q.shape[:2]
-        self._heads("q", q, n, heads)
+        n, heads = q.shape[0], q.shape[1]
+        a = KvAttend()
+        a.q_stride = self._heads("q", q, n, heads)
         self._on("block_table", block_table, torch.int32, 2)
-        if block_table.shape[0] != n or block_table.shape[1] < 1 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        (rows, width), stride = block_table.shape, block_table.stride()
+        if rows != n or width < 1 or (width > 1 and stride[1] != 1):
             raise ValueError(f"block_table must be {n} rows of contiguous entries")
-        self._flat("seq_lens", seq_lens, torch.int32, n)
+        a.seq_lens = self._flat("seq_lens", seq_lens, torch.int32, n)
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
-        if out is not None:
-            self._heads("out", out, n, heads)
-
-        def call(s):
-            o = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device) if out is None else out
-            lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
-            if n:
-                a = KvAttend(q=q.data_ptr(), out=o.data_ptr(), lse=None if lse is None else lse.data_ptr(),
-                             block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(), table_stride=block_table.stride(0),
-                             window=window, sinks=sinks, batch=n, n_q_heads=heads, table_width=block_table.shape[1],
-                             scale=self.head_dim ** -0.5 if scale is None else scale)
-                a.q_stride[:], a.out_stride[:] = q.stride()[:2], o.stride()[:2]
-                scratch = self._scratch()
-                check(self.lib.bam_launch_kv_attend(self.array.h, self._layout(layer), C.byref(a), scratch.data_ptr(),
-                                                    self._scratch_bytes, s), "bam_launch_kv_attend")
-            return (o, lse) if return_lse else o
-        self._layout(layer)
-        return self._run(stream, call)
+        layout = self._layout(layer)
+        if out is None:
+            out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
+        a.out_stride = self._heads("out", out, n, heads)
+        lse = None
+        if return_lse:
+            lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
+            a.lse = lse.data_ptr()
+        a.q, a.out, a.block_table, a.table_stride = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), stride[0]
+        a.window, a.sinks, a.batch, a.n_q_heads, a.table_width = window, sinks, n, heads, width
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        if n:
+            self._call("bam_launch_kv_attend", layout, C.byref(a))
+        return (out, lse) if return_lse else out
