@@ -175,6 +175,8 @@ struct KvAppendWork {
     const uint16_t *q_norm, *k_norm;
     float eps, inv_dim;
 
+    BAM_DEV uint32_t counters(uint32_t) const { return 0; }
+
     /* the position of a token, or -1 after the error has been recorded */
     BAM_DEV int64_t position(uint64_t t, bool padded) const
     {
@@ -341,6 +343,8 @@ struct KvGatherWork {
     uint32_t lanes_per_row, tokens_per_item;
     const int64_t* slots;
 
+    BAM_DEV uint32_t counters(uint32_t) const { return 0; }
+
     __device__ void operator()(uint32_t vb, uint32_t nvb) const
     {
         const uint32_t lane = threadIdx.x & 31u;
@@ -447,6 +451,17 @@ extern "C" uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* l
     return kv_parts_at(most * KV_WORKERS) + (uint64_t)most * KV_WORKERS * 2 * KV_ROWS * (L.head_dim + 2) * sizeof(float);
 }
 
+extern "C" int bam_kv_scratch_init(bam_array_t a, void* scratch_dev, uint64_t scratch_bytes, void* stream)
+{
+    if (!a || !scratch_dev || ((uintptr_t)scratch_dev & 127)) return BAM_EINVAL;
+    const uint64_t head = kv_parts_at(kv_most_blocks(a) * KV_WORKERS);
+    if (scratch_bytes < head) return BAM_EINVAL;
+    device_guard g;
+    CK(g.enter(a->pc->ctrl->device));
+    CK(cudaMemsetAsync(scratch_dev, 0xff, head, (cudaStream_t)stream));
+    return BAM_OK;
+}
+
 static int check_scratch(bam_array_t a, const bam_kv_layout_t* layout, void* scratch, uint64_t scratch_bytes)
 {
     if (!scratch || ((uintptr_t)scratch & 127)) return BAM_EINVAL;
@@ -474,7 +489,7 @@ static int launch_append_as(bam_array_t a, const kv_layout_d_t& L, const bam_kv_
     w.rope.stride = p->rope_stride; w.rope.rotary_dim = p->cos ? p->rotary_dim : 0; w.rope.style = p->rope_style;
     w.q_norm = (const uint16_t*)p->q_norm; w.k_norm = (const uint16_t*)p->k_norm; w.eps = p->norm_eps; w.inv_dim = 1.f / (float)L.head_dim;
     const uint64_t items = (p->n_tokens + w.k_tokens - 1) / w.k_tokens * w.k_parts + (p->n_tokens + w.q_tokens - 1) / w.q_tokens * w.q_parts;
-    return kv_launch(a->pc->ctrl, w, items, scratch, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+    return kv_launch(a->pc->ctrl, w, items, scratch, (cudaStream_t)stream);
 }
 
 template <class T>
@@ -524,7 +539,7 @@ static int launch_gather(bam_array_t a, const kv_layout_d_t& L, uint64_t n_token
     w.tokens_per_item = tokens_of_item(n_tokens, L.n_kv_heads, warps, KV_MAX_LANE_TOKENS);
     w.slots = slots_dev;
     const uint64_t items = (n_tokens + w.tokens_per_item - 1) / w.tokens_per_item * L.n_kv_heads;
-    return kv_launch(a->pc->ctrl, w, items, scratch, sizeof(kv_launch_words_t), (cudaStream_t)stream);
+    return kv_launch(a->pc->ctrl, w, items, scratch, (cudaStream_t)stream);
 }
 
 extern "C" int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t n_tokens, const int64_t* slots_dev,

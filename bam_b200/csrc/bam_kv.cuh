@@ -26,14 +26,16 @@ namespace bam {
 #define KV_WORKERS 3u                 /* worker warps of a block of the attention; with the fourth, which only a controller
                                        * block uses, a thread may have 255 registers */
 
-/* A launch's own words at the head of its scratch, all ones when the launch starts (one memset, so a captured
- * launch needs no host memory): `remaining` is what the controller blocks watch, `done` counts worker blocks down,
- * `drawn` counts the items that were drawn.
- * An index outside its range is noted in `bad_index`, bit 31 of `done` tells of it, and it goes into the status block by
- * the last worker block: a status that is set earlier makes every wait of the launch give up, and a page whose fetch is
- * given up is lost to the cache. */
+/* A launch's own words at the head of its scratch.  They (and the counters behind them) are all ones when a launch starts,
+ * and the last of its blocks leaves them so for the next one that uses the scratch: no memset per launch.
+ *   remaining  what the controller blocks watch; the last worker block clears it
+ *   left       counts down.  Bits 0-14: worker blocks; bit 15: cleared when an index was outside its range; bits 16-31: all
+ *              blocks.  (An index outside its range is noted in bad_index and goes into the status block by the last worker
+ *              block: a status that is set earlier makes every wait of the launch give up, and a page whose fetch is given
+ *              up is lost to the cache.)
+ *   drawn      items that were drawn */
 struct kv_launch_words_t {
-    uint32_t remaining, done;
+    uint32_t remaining, left;
     uint64_t bad_index;
     uint32_t drawn, pad[11];
 };
@@ -50,7 +52,7 @@ struct kv_layout_d_t {
     BAM_DEV void bad_index(uint64_t i) const
     {
         st_relaxed_gpu(&words->bad_index, i);
-        (void)atom_and_release(&words->done, 0x7fffffffu);
+        (void)atom_and_release(&words->left, ~0x8000u);
     }
     /* the number of draws before this one; a warp draws together */
     BAM_DEV uint32_t draw() const
@@ -118,32 +120,39 @@ BAM_DEV void kv_store8(uint16_t* p, uint4 v, bool vec)
     for (int i = 0; i < 4; i++) { p[2 * i] = (uint16_t)w[i]; p[2 * i + 1] = (uint16_t)(w[i] >> 16); }
 }
 
-/* The fused launch of these operators.  Like bam_fused, but the words that end the controller blocks belong to
- * the launch and not to the controller, so that launches on one controller may overlap and a captured launch can
- * be replayed: worker blocks count down from all-ones, and the last one clears `remaining`. */
+/* The fused launch of these operators.  Like bam_fused, but the words that end the controller blocks belong to the launch
+ * and not to the controller, so that launches on one controller may overlap and a captured launch can be replayed.
+ * Work::counters() of the words behind the launch's own are the workload's. */
 template <class Work>
 __global__ void __launch_bounds__(Work::threads, Work::min_blocks)
 bam_kv_fused(const __grid_constant__ bam_emu_d_t emu, const __grid_constant__ Work work)
 {
-    if (blockIdx.x < emu.n_ctrl_blocks) {
-        emu_controller_main(emu, bam_dyn_smem);
-        return;
-    }
+    kv_launch_words_t* const words = reinterpret_cast<kv_launch_words_t*>(emu.consumers_remaining);
+    const bool controls = blockIdx.x < emu.n_ctrl_blocks;
     const uint32_t n_work = gridDim.x - emu.n_ctrl_blocks;
-    work(blockIdx.x - emu.n_ctrl_blocks, n_work);
+    if (controls) emu_controller_main(emu, bam_dyn_smem);
+    else work(blockIdx.x - emu.n_ctrl_blocks, n_work);
     __syncthreads();
+    /* (in the dynamic shared memory, which nobody uses any more: 128 bytes of their own would take three blocks of the gather
+     * over 196 KB an SM, and half of the L1 with it: 55 -> 60 us) */
+    uint32_t* const old_left = reinterpret_cast<uint32_t*>(bam_dyn_smem);
     if (threadIdx.x == 0) {
         /* nothing is published here: what the launch wrote becomes visible with its end */
-        kv_launch_words_t* w = reinterpret_cast<kv_launch_words_t*>(emu.consumers_remaining);
-        const uint32_t left = atom_add_relaxed(&w->done, 0xffffffffu);
-        if ((left & 0x7fffffffu) == 0x80000000u - n_work) {                       /* the last of them */
-            if (!(left & 0x80000000u)) {
+        const uint32_t old = atom_add_relaxed(&words->left, controls ? 0u - 0x10000u : 0u - 0x10001u);
+        if (!controls && (old & 0x7fffu) == 0x8000u - n_work) {                       /* the last of the workers */
+            if (!(old & 0x8000u)) {
                 fence_acq_rel_gpu();
-                status_fail(emu.status, BAM_ERANGE, BAM_AT_RANGE, ld_relaxed_gpu(&w->bad_index));
+                status_fail(emu.status, BAM_ERANGE, BAM_AT_RANGE, ld_relaxed_gpu(&words->bad_index));
             }
-            st_release_scoped(&w->remaining, 0u, emu.sys_scope != 0);
+            st_release_scoped(&words->remaining, 0u, emu.sys_scope != 0);
         }
+        *old_left = old;
     }
+    __syncthreads();
+    if ((*old_left >> 16) != 0x10000u - gridDim.x) return;
+    /* the last block of all: nobody reads or writes the words any more (whether the launch succeeded or was given up) */
+    uint32_t* w = reinterpret_cast<uint32_t*>(words);
+    for (uint32_t i = threadIdx.x; i < sizeof(kv_launch_words_t) / 4 + work.counters(n_work); i += blockDim.x) w[i] = 0xffffffffu;
 }
 
 /* ---- host side ------------------------------------------------------------------------------------------ */
@@ -181,10 +190,9 @@ cudaError_t kv_max_grid(int dev, uint32_t* grid)
     return cudaSuccess;
 }
 
-/* Launch with at most `want` worker blocks.  The launch's words are the first bytes of `scratch`; `clear` bytes of
- * it are set to all ones. */
+/* Launch with at most `want` worker blocks.  The launch's words are the first bytes of `scratch`. */
 template <class Work>
-int kv_launch(bam_ctrl* c, const Work& work, uint64_t want, void* scratch, size_t clear, cudaStream_t s)
+int kv_launch(bam_ctrl* c, const Work& work, uint64_t want, void* scratch, cudaStream_t s)
 {
     uint32_t grid = 0;
     CK(kv_max_grid<Work>(c->device, &grid));
@@ -200,7 +208,6 @@ int kv_launch(bam_ctrl* c, const Work& work, uint64_t want, void* scratch, size_
     emu.consumers_remaining = reinterpret_cast<uint32_t*>(scratch);
     Work w = work;
     w.L.words = reinterpret_cast<kv_launch_words_t*>(scratch);
-    CK(cudaMemsetAsync(scratch, 0xff, clear, s));
     void* args[] = { (void*)&emu, (void*)&w };
     CK(cudaLaunchCooperativeKernel((const void*)bam_kv_fused<Work>, dim3(grid), dim3(Work::threads), args, Work::smem, s));
     return BAM_OK;

@@ -121,6 +121,7 @@ struct KvAttendWork {
     uint32_t* arrived;                                   /* per worker, all ones at the start: arrivals at the unit it begins */
     float* parts;                                        /* [worker][2]: rows x head_dim sums, 16 maxima, 16 denominators */
 
+    BAM_DEV uint32_t counters(uint32_t blocks) const { return blocks * KV_WORKERS; }
     BAM_DEV uint32_t dim() const { return EXACT ? (uint32_t)DMAX : L.head_dim; }
     BAM_DEV uint32_t row_bytes() const { return dim() * 2u; }
     BAM_DEV uint32_t stage_bytes() const { return CS * dim() * 4u; }
@@ -898,7 +899,7 @@ static int launch_attend_nt(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
      * full for that makes the pinning warps ask for less) */
     const uint64_t share = a->pc->d.n_slots / (blocks * KV_WORKERS * (CS / w.piece));
     w.ahead = share < 2 ? 2u : share < KV_AHEAD ? (uint32_t)share : KV_AHEAD;
-    return kv_launch(a->pc->ctrl, w, blocks, scratch, sizeof(kv_launch_words_t) + 4 * (size_t)most * KV_WORKERS, (cudaStream_t)stream);
+    return kv_launch(a->pc->ctrl, w, blocks, scratch, (cudaStream_t)stream);
 }
 
 template <class T, int DMAX, int CS, bool EXACT>

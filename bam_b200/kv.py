@@ -13,6 +13,15 @@ from .host import REPLICATE, Array
 
 ROPE_STYLES = {"half": 0, "pairs": 1}
 
+_scratch = {}       # (device, stream) -> the scratch memory of the launches on that stream
+
+
+def _raw_stream(index):
+    """The handle of torch's current stream (by the short way where this torch has it: a call takes 15 us in all)."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+
 
 class KvCache:
     """n_layers x n_blocks blocks of block_tokens tokens for n_kv_heads heads of head_dim elements.
@@ -90,13 +99,24 @@ class KvCache:
             raise ValueError(f"the stream is on {stream.device}, the cache on {self.device}")
         return torch.cuda.stream(stream)
 
-    def _call(self, name, layer, *args):
-        """A launch on the current stream of the cache's device, with scratch memory of its own (so that calls on other
-        streams and captured ones, whose scratch belongs to their graph, do not meet in it)."""
+    def _call(self, launch, layer, *args):
+        """A launch on the current stream of the cache's device.  Scratch memory belongs to the stream, whose launches run
+        one after the other (and share it between all caches of the device); a captured launch has its own, which belongs
+        to its graph."""
         import torch
-        scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=self.device)
-        check(getattr(self.lib, name)(self.array.h, layer, *args, scratch.data_ptr(), self._scratch_bytes,
-                                      torch.cuda.current_stream(self.device.index).cuda_stream), name)
+        index = self.device.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                return self._call(launch, layer, *args)
+        stream = _raw_stream(index)
+        capturing = torch.cuda.is_current_stream_capturing()
+        scratch = None if capturing else _scratch.get((index, stream))
+        if scratch is None or scratch.numel() < self._scratch_bytes:
+            scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+            check(self.lib.bam_kv_scratch_init(self.array.h, scratch.data_ptr(), self._scratch_bytes, stream), "bam_kv_scratch_init")
+            if not capturing:
+                _scratch[index, stream] = scratch
+        check(launch(self.array.h, layer, *args, scratch.data_ptr(), self._scratch_bytes, stream), launch.__name__)
 
     # ---- operators ----------------------------------------------------------------------------------------
 
@@ -153,10 +173,12 @@ class KvCache:
             a.q_stride = self._heads("q", q, n, a.n_q_heads)
             if q_out is None:
                 q_out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-            a.q_out_stride = self._heads("q_out", q_out, n, a.n_q_heads)
+                a.q_out_stride = a.n_q_heads * self.head_dim, self.head_dim
+            else:
+                a.q_out_stride = self._heads("q_out", q_out, n, a.n_q_heads)
             a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
         if n:
-            self._call("bam_launch_kv_append", layout, C.byref(a))
+            self._call(self.lib.bam_launch_kv_append, layout, C.byref(a))
         return q_out
 
     def gather(self, slots, layer=0, out=None, stream=None):
@@ -170,13 +192,14 @@ class KvCache:
         at = self._flat("slots", slots, torch.int64, n)
         layout = self._layout(layer)
         if out is None:
-            shape = (n, self.n_kv_heads, self.head_dim)
-            out = (torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device))
-        k, v = out
-        ks = (C.c_int64 * 2)(*self._heads("out[0]", k, n, self.n_kv_heads))
-        vs = (C.c_int64 * 2)(*self._heads("out[1]", v, n, self.n_kv_heads))
+            k, v = torch.empty((2, n, self.n_kv_heads, self.head_dim), dtype=self.dtype, device=self.device).unbind()
+            ks = vs = (C.c_int64 * 2)(self.n_kv_heads * self.head_dim, self.head_dim)
+        else:
+            k, v = out
+            ks = (C.c_int64 * 2)(*self._heads("out[0]", k, n, self.n_kv_heads))
+            vs = (C.c_int64 * 2)(*self._heads("out[1]", v, n, self.n_kv_heads))
         if n:
-            self._call("bam_launch_kv_gather", layout, n, at, k.data_ptr(), v.data_ptr(), ks, vs)
+            self._call(self.lib.bam_launch_kv_gather, layout, n, at, k.data_ptr(), v.data_ptr(), ks, vs)
         return k, v
 
     def attend(self, q, block_table, seq_lens, layer=0, scale=None, window=0, sinks=0, out=None, return_lse=False, stream=None):
@@ -206,7 +229,9 @@ class KvCache:
         layout = self._layout(layer)
         if out is None:
             out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
-        a.out_stride = self._heads("out", out, n, heads)
+            a.out_stride = heads * self.head_dim, self.head_dim
+        else:
+            a.out_stride = self._heads("out", out, n, heads)
         lse = None
         if return_lse:
             lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
@@ -215,5 +240,5 @@ class KvCache:
         a.window, a.sinks, a.batch, a.n_q_heads, a.table_width = window, sinks, n, heads, width
         a.scale = self.head_dim ** -0.5 if scale is None else scale
         if n:
-            self._call("bam_launch_kv_attend", layout, C.byref(a))
+            self._call(self.lib.bam_launch_kv_attend, layout, C.byref(a))
         return (out, lse) if return_lse else out

@@ -363,9 +363,9 @@ int bam_ctrl_write_store_from_device(bam_ctrl_t c, uint64_t byte_offset, const v
  * head_dim: a multiple of 16, at most 256; block_tokens: a multiple of 16 with block_tokens * head_dim * 4 <= the page.
  * Strides are in elements: [0] from token (or sequence) to token, [1] from head to head; a head's elements are
  * contiguous.  Every launch is asynchronous on `stream`, may be captured into a CUDA graph, and leaves the calling
- * thread's device as it was.  scratch_dev: bam_kv_scratch_bytes bytes of device memory, 128-byte aligned, that nothing
- * else uses until the launch has finished (a captured launch keeps using it: every graph needs its own); its contents
- * need no initialisation.  An index outside its range (a slot, position, block or length) is not followed: the status
+ * thread's device as it was.  scratch_dev: bam_kv_scratch_bytes bytes of device memory, 128-byte aligned, set up once
+ * by bam_kv_scratch_init.  Every launch leaves it ready for the next, also one that fails; launches that may run at the
+ * same time need one each: one for every stream, one for every captured graph.  An index outside its range (a slot, position, block or length) is not followed: the status
  * block says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has finished, the rows that it concerns are undefined. */
 #define BAM_KV_BF16 0u
 #define BAM_KV_FP16 1u
@@ -377,6 +377,7 @@ typedef struct {
     uint64_t first_page;         /* page of the array that block 0, head 0 is (a layer's share of the array starts there) */
 } bam_kv_layout_t;
 uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* layout);
+int bam_kv_scratch_init(bam_array_t a, void* scratch_dev, uint64_t scratch_bytes, void* stream);
 
 /* Append: row t of k and v goes to slots[t] (int64; negative: the row is padding and nothing is written; slots are
  * distinct otherwise: of two rows for one slot neither is sure to be kept whole).  On the way each head of k, and of q where it is given, is

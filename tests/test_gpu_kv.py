@@ -435,6 +435,9 @@ def test_c_entries_refuse(cuda, bam):
     EINVAL, ERANGE = 22, 34
     scratch = torch.empty(kv._scratch_bytes + 256, dtype=torch.uint8, device="cuda")
     sp, sb = scratch.data_ptr(), kv._scratch_bytes
+    assert lib.bam_kv_scratch_init(None, sp, sb, None) == EINVAL and lib.bam_kv_scratch_init(h, None, sb, None) == EINVAL
+    assert lib.bam_kv_scratch_init(h, sp + 64, sb, None) == EINVAL and lib.bam_kv_scratch_init(h, sp, 64, None) == EINVAL
+    assert lib.bam_kv_scratch_init(h, sp, sb, None) == 0
     t = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
     i64, i32, f = (torch.zeros(64, dtype=d, device="cuda") for d in (torch.int64, torch.int32, torch.float32))
     good = dict(dtype=0, head_dim=64, n_kv_heads=2, block_tokens=16, n_blocks=10, first_page=0)

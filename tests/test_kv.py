@@ -12,6 +12,7 @@ def test_c_entries_refuse_missing_handles(bam):
     layout = _lib.KvLayout(0, 64, 2, 16, 8, 0)
     two = (C.c_int64 * 2)(0, 0)
     assert lib.bam_kv_scratch_bytes(None, C.byref(layout)) == 0
+    assert lib.bam_kv_scratch_init(None, None, 0, None) == EINVAL
     assert lib.bam_launch_kv_append(None, C.byref(layout), C.byref(_lib.KvAppend()), None, 0, None) == EINVAL
     assert lib.bam_launch_kv_gather(None, C.byref(layout), 1, None, None, None, two, two, None, 0, None) == EINVAL
     assert lib.bam_launch_kv_attend(None, C.byref(layout), C.byref(_lib.KvAttend()), None, 0, None) == EINVAL
