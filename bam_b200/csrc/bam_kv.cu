@@ -8,6 +8,7 @@
  */
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstring>
 
 #include "bam_kv.cuh"
@@ -511,7 +512,7 @@ extern "C" int bam_launch_kv_append(bam_array_t a, const bam_kv_layout_t* layout
     if (p->q && (!p->q_out || p->n_q_heads == 0 || p->n_q_heads > 65536)) return BAM_EINVAL;
     if (p->cos || p->sin) {
         if (!p->cos || !p->sin || !p->positions || p->n_positions == 0 || p->n_positions > 0x7fffffffffffull) return BAM_EINVAL;
-        if (p->rotary_dim == 0 || p->rotary_dim > L.head_dim || p->rotary_dim % 16 || p->rope_stride < p->rotary_dim / 2) return BAM_EINVAL;
+        if (p->rotary_dim == 0 || p->rotary_dim > L.head_dim || p->rotary_dim % 16 || p->rope_stride < 0) return BAM_EINVAL;
         if (p->rope_style != BAM_KV_ROPE_HALF && p->rope_style != BAM_KV_ROPE_PAIRS) return BAM_EINVAL;
     }
     if ((p->q_norm || p->k_norm) && !(p->norm_eps >= 0.f)) return BAM_EINVAL;
@@ -569,7 +570,7 @@ extern "C" int bam_launch_kv_attend(bam_array_t a, const bam_kv_layout_t* layout
     if (!p || !p->q || !p->out || !p->block_table || !p->seq_lens) return BAM_EINVAL;
     if (p->n_q_heads == 0 || p->n_q_heads > 65536 || p->n_q_heads % L.n_kv_heads) return BAM_EINVAL;
     if (p->batch > (1u << 20) || p->table_width == 0 || p->table_width > (1u << 27) || p->window < 0 || p->sinks < 0) return BAM_EINVAL;
-    if (!(p->scale == p->scale)) return BAM_EINVAL;
+    if (!std::isfinite(p->scale)) return BAM_EINVAL;
     rc = check_scratch(a, layout, scratch_dev, scratch_bytes);
     if (rc) return rc;
     if (p->batch == 0) return BAM_OK;

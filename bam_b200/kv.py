@@ -157,7 +157,7 @@ class KvCache:
             if rotary % 16 or not 0 < rotary <= self.head_dim:
                 raise ValueError(f"{rotary} rotated elements: a multiple of 16 up to {self.head_dim} is wanted")
             a.cos, a.sin, a.n_positions = cos.data_ptr(), sin.data_ptr(), rows
-            a.rope_stride, a.rotary_dim, a.rope_style = max(stride[0], half), rotary, ROPE_STYLES[rope_style]
+            a.rope_stride, a.rotary_dim, a.rope_style = stride[0], rotary, ROPE_STYLES[rope_style]
         if q_norm is not None:
             a.q_norm = self._flat("q_norm", q_norm, self.dtype, self.head_dim)
         if k_norm is not None:
@@ -237,7 +237,8 @@ class KvCache:
             lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
             a.lse = lse.data_ptr()
         a.q, a.out, a.block_table, a.table_stride = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), stride[0]
-        a.window, a.sinks, a.batch, a.n_q_heads, a.table_width = window, sinks, n, heads, width
+        a.window, a.sinks = min(window, 1 << 62), min(sinks, 1 << 62)
+        a.batch, a.n_q_heads, a.table_width = n, heads, width
         a.scale = self.head_dim ** -0.5 if scale is None else scale
         if n:
             self._call(self.lib.bam_launch_kv_attend, layout, C.byref(a))

@@ -462,7 +462,7 @@ def test_c_entries_refuse(cuda, bam):
     assert append() == 0 and append(**rope) == 0 and append(n_tokens=0) == 0
     for c in (dict(k=None), dict(v=None), dict(slots=None), dict(n_tokens=1 << 31), dict(q=t.data_ptr()), dict(scratch=None), dict(scratch=sp + 64),
               dict(size=sb - 1), dict(rope, sin=None), dict(rope, positions=None), dict(rope, n_positions=0), dict(rope, rotary_dim=24),
-              dict(rope, rotary_dim=80), dict(rope, rope_stride=31), dict(rope, rope_style=2), dict(k_norm=t.data_ptr(), norm_eps=-1.0),
+              dict(rope, rotary_dim=80), dict(rope, rope_stride=-1), dict(rope, rope_style=2), dict(k_norm=t.data_ptr(), norm_eps=-1.0),
               dict(k_norm=t.data_ptr(), norm_eps=float("nan")), dict(q=t.data_ptr(), q_out=t.data_ptr(), n_q_heads=0)):
         assert append(**c) == EINVAL, c
     at = dict(q=t.data_ptr(), out=t.data_ptr(), q_stride=(128, 64), out_stride=(128, 64), block_table=i32.data_ptr(), seq_lens=i32.data_ptr(),
@@ -478,7 +478,7 @@ def test_c_entries_refuse(cuda, bam):
         return lib.bam_launch_kv_attend(h, L(), C.byref(a), scratch, size, None)
     assert attend() == 0 and attend(batch=0) == 0
     for c in (dict(q=None), dict(out=None), dict(block_table=None), dict(seq_lens=None), dict(n_q_heads=3), dict(n_q_heads=0), dict(table_width=0),
-              dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(batch=(1 << 20) + 1), dict(size=0), dict(scratch=None)):
+              dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=(1 << 20) + 1), dict(size=0), dict(scratch=None)):
         assert attend(**c) == EINVAL, c
     # an array that starts inside a page is refused
     a2 = bam.Array.from_ranges(kv.cache, 512, [(0, 512, 0, 64)])
@@ -669,4 +669,84 @@ def test_empty_calls(cuda, bam):
     pads = torch.full((3,), -1, dtype=torch.int64, device="cuda")
     kv.append(q, q, pads)
     assert kv.cache.stats()["accesses"] == 0
+    done(kv)
+
+
+def test_more_heads_than_lanes_and_angles_of_one_row(cuda, bam):
+    """40 key/value heads; angles that are one row for all positions; a page that its block does not fill; windows and
+    numbers of first tokens beyond any length."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(12)
+    H, D = 40, 32
+    kv = make(bam, torch, 9, H, D, torch.bfloat16, page=8192, tokens=48)
+    T = 48
+    lens = [100, 48, 5, 0, 47]
+    k, v, table = fill(torch, g, kv, lens, spare=0)
+    n = len(k)
+    row = torch.rand(1, D // 2, generator=g, device="cuda")
+    cos, sin = row.expand(n, -1), row.expand(n, -1)
+    q = rand(torch, g, n, H, D, dtype=torch.bfloat16)
+    at = torch.arange(n, device="cuda")
+    got = kv.append(k, v, at, positions=at, rope=(cos, sin), q=q)
+    wq, mq = transform64(torch, q, None, 0, cos, sin, "half")
+    close_transform(torch, got, wq, mq, D, torch.bfloat16)
+    wk, mk = transform64(torch, k, None, 0, cos, sin, "half")
+    bk, bv = kv.gather(at)
+    close_transform(torch, bk, wk, mk, D, torch.bfloat16)
+    assert torch.equal(bv, v)
+    q = rand(torch, g, len(lens), 2 * H, D, dtype=torch.bfloat16, scale=2.0)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = attend64(torch, q, bk, bv, table, lens, T, D ** -0.5)
+    for window, sinks in ((0, 0), (1 << 70, 0), (3, 1 << 70), (100, 0)):
+        out, lse = kv.attend(q, table, ls, window=window, sinks=sinks, return_lse=True)
+        check_attend(torch, out, lse, ref, torch.bfloat16)
+    assert kv.cache.ctrl.status() == (0, "none", 0)
+    done(kv)
+
+
+def test_values_that_are_not_finite_in_visible_rows(cuda, bam):
+    """A score of +infinity or NaN makes its row NaN, as the formula has it; -infinity hides its token; other sequences and
+    heads do not notice."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(13)
+    lens = [70, 70, 70, 40]
+    kv = make(bam, torch, 24, 1, 64, torch.bfloat16, page=4096)
+    k, v, table = fill(torch, g, kv, lens)
+    T = kv.block_tokens
+    k = k.abs()
+    at = lambda b, j: table[b].long()[j // T] * T + j % T           # noqa: E731
+    k[at(0, 33), 0, 5] = float("inf")
+    k[at(1, 69), 0, 5] = float("nan")
+    k[at(2, 10), 0, 5] = float("-inf")
+    v[at(2, 10)] = 3.0
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    q = rand(torch, g, 4, 2, 64, dtype=torch.bfloat16).abs() + 0.25
+    out, lse = kv.attend(q.bfloat16(), table, torch.tensor(lens, dtype=torch.int32, device="cuda"), return_lse=True)
+    assert torch.isnan(out[:2]).all() and torch.isnan(lse[:2]).all()
+    k[at(2, 10), 0, 5] = -1e30                                         # hidden all the same, and finite in 64 bits
+    ref = attend64(torch, q.bfloat16()[2:], k, v, table[2:], lens[2:], T, 0.125)
+    err = (out[2:].double() - ref[0]).abs()
+    assert (err <= 2.0 ** -7 * ref[0].abs() + 2.0 ** -7).all()
+    done(kv)
+
+
+def test_offsets_beyond_32_bits(cuda, bam):
+    """More than 4 GiB of cache memory and of store: one token in every page of a megabyte, read back and attended to."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(14)
+    blocks, D, page = 4400, 256, 1 << 20
+    kv = make(bam, torch, blocks, 1, D, torch.bfloat16, page=page)
+    T = kv.block_tokens
+    assert T == 1024
+    first = torch.arange(blocks, device="cuda") * T
+    k, v = rand(torch, g, blocks, 1, D, dtype=torch.bfloat16), rand(torch, g, blocks, 1, D, dtype=torch.bfloat16)
+    kv.append(k, v, first)
+    assert kv.cache.ctrl.status() == (0, "none", 0)
+    bk, bv = kv.gather(first.flip(0))
+    assert torch.equal(bk, k.flip(0)) and torch.equal(bv, v.flip(0))
+    table = torch.tensor([[blocks - 1], [blocks - 2], [0]], dtype=torch.int32, device="cuda")
+    q = rand(torch, g, 3, 2, D, dtype=torch.bfloat16)
+    out = kv.attend(q, table, torch.ones(3, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out, v[table[:, 0].long()].expand(3, 2, D))     # one visible token: its value
+    assert kv.cache.ctrl.status() == (0, "none", 0)
     done(kv)
