@@ -13,6 +13,7 @@ from .host import REPLICATE, Array
 
 ROPE_STYLES = {"half": 0, "pairs": 1}
 
+_NO_STRIDE = (0, 0)
 _scratch = {}       # (device, stream) -> the scratch memory of the launches on that stream
 
 
@@ -75,8 +76,10 @@ class KvCache:
 
     def _heads(self, name, t, n, heads):
         """The strides of a tensor [n, heads, head_dim] whose heads are contiguous."""
-        self._on(name, t, self.dtype, 3)
         shape, stride = t.shape, t.stride()
+        if t.dtype is self.dtype and shape == (n, heads, self.head_dim) and stride[2] == 1 and t.device == self.device:
+            return stride[:2]
+        self._on(name, t, self.dtype, 3)
         if (n is not None and shape[0] != n) or shape[1] != heads or shape[2] != self.head_dim:
             raise ValueError(f"{name} has shape {tuple(shape)}, wanted ({'n' if n is None else n}, {heads}, {self.head_dim})")
         if stride[2] != 1:
@@ -85,9 +88,10 @@ class KvCache:
 
     def _flat(self, name, t, dtype, n):
         """The address of n contiguous values."""
-        self._on(name, t, dtype, 1)
-        if t.shape[0] != n or (n > 1 and t.stride(0) != 1):
-            raise ValueError(f"{name} must be {n} contiguous values")
+        if not (t.dtype is dtype and t.shape == (n,) and t.is_contiguous() and t.device == self.device):
+            self._on(name, t, dtype, 1)
+            if t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+                raise ValueError(f"{name} must be {n} contiguous values")
         return t.data_ptr()
 
     def _on_stream(self, stream):
@@ -136,11 +140,9 @@ class KvCache:
             with self._on_stream(stream):
                 return self.append(k, v, slots, layer, positions, rope, rope_style, q, q_norm, k_norm, norm_eps, q_out)
         n = k.shape[0]
-        a = KvAppend()
-        a.k_stride = self._heads("k", k, None, self.n_kv_heads)
-        a.v_stride = self._heads("v", v, n, self.n_kv_heads)
-        a.slots = self._flat("slots", slots, torch.int64, n)
-        a.k, a.v, a.n_tokens, a.norm_eps = k.data_ptr(), v.data_ptr(), n, norm_eps
+        k_stride, v_stride = self._heads("k", k, n, self.n_kv_heads), self._heads("v", v, n, self.n_kv_heads)
+        at = self._flat("slots", slots, torch.int64, n)
+        turn = 0, 0, 0, 0, 0, 0, 0                       # positions, cos, sin, rows, their stride, rotated elements, style
         if rope is not None:
             cos, sin = rope
             self._on("cos", cos, torch.float32, 2)
@@ -149,35 +151,35 @@ class KvCache:
                 raise ValueError(f"rope_style must be one of {sorted(ROPE_STYLES)}, not {rope_style!r}")
             if positions is None:
                 raise ValueError("a rotation needs positions")
-            a.positions = self._flat("positions", positions, torch.int64, n)
             (rows, half), stride = cos.shape, cos.stride()
             if sin.shape != cos.shape or sin.stride() != stride or stride[1] != 1 or rows == 0:
                 raise ValueError("cos and sin must be rows of the same shape and strides")
-            rotary = 2 * half
-            if rotary % 16 or not 0 < rotary <= self.head_dim:
-                raise ValueError(f"{rotary} rotated elements: a multiple of 16 up to {self.head_dim} is wanted")
-            a.cos, a.sin, a.n_positions = cos.data_ptr(), sin.data_ptr(), rows
-            a.rope_stride, a.rotary_dim, a.rope_style = stride[0], rotary, ROPE_STYLES[rope_style]
-        if q_norm is not None:
-            a.q_norm = self._flat("q_norm", q_norm, self.dtype, self.head_dim)
-        if k_norm is not None:
-            a.k_norm = self._flat("k_norm", k_norm, self.dtype, self.head_dim)
+            if half % 8 or not 0 < 2 * half <= self.head_dim:
+                raise ValueError(f"{2 * half} rotated elements: a multiple of 16 up to {self.head_dim} is wanted")
+            turn = (self._flat("positions", positions, torch.int64, n), cos.data_ptr(), sin.data_ptr(), rows, stride[0], 2 * half,
+                    ROPE_STYLES[rope_style])
+        q_w = None if q_norm is None else self._flat("q_norm", q_norm, self.dtype, self.head_dim)
+        k_w = None if k_norm is None else self._flat("k_norm", k_norm, self.dtype, self.head_dim)
         layout = self._layout(layer)
+        q_at = out_at = None
+        heads, q_stride, out_stride = 0, _NO_STRIDE, _NO_STRIDE
         if q is None:
             if q_norm is not None or q_out is not None:
                 raise ValueError("q_norm and q_out go with q")
         else:
             if q.dim() != 3 or q.shape[1] < 1:
                 raise ValueError("q must be [n, heads, head_dim]")
-            a.n_q_heads = q.shape[1]
-            a.q_stride = self._heads("q", q, n, a.n_q_heads)
+            heads = q.shape[1]
+            q_stride = self._heads("q", q, n, heads)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-                a.q_out_stride = a.n_q_heads * self.head_dim, self.head_dim
+                q_out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
+                out_stride = heads * self.head_dim, self.head_dim
             else:
-                a.q_out_stride = self._heads("q_out", q_out, n, a.n_q_heads)
-            a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+                out_stride = self._heads("q_out", q_out, n, heads)
+            q_at, out_at = q.data_ptr(), q_out.data_ptr()
         if n:
+            a = KvAppend(q_at, k.data_ptr(), v.data_ptr(), out_at, q_stride, k_stride, v_stride, out_stride, n, at, *turn[:5],
+                         q_w, k_w, heads, turn[5], turn[6], norm_eps)
             self._call(self.lib.bam_launch_kv_append, layout, C.byref(a))
         return q_out
 
@@ -217,29 +219,24 @@ class KvCache:
         if q.dim() != 3 or q.shape[1] < 1 or q.shape[1] % self.n_kv_heads:
             raise ValueError(f"q must be [batch, heads, head_dim] with a multiple of {self.n_kv_heads} heads")
         n, heads = q.shape[0], q.shape[1]
-        a = KvAttend()
-        a.q_stride = self._heads("q", q, n, heads)
+        q_stride = self._heads("q", q, n, heads)
         self._on("block_table", block_table, torch.int32, 2)
         (rows, width), stride = block_table.shape, block_table.stride()
         if rows != n or width < 1 or (width > 1 and stride[1] != 1):
             raise ValueError(f"block_table must be {n} rows of contiguous entries")
-        a.seq_lens = self._flat("seq_lens", seq_lens, torch.int32, n)
+        lens = self._flat("seq_lens", seq_lens, torch.int32, n)
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
         layout = self._layout(layer)
         if out is None:
             out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
-            a.out_stride = heads * self.head_dim, self.head_dim
+            out_stride = heads * self.head_dim, self.head_dim
         else:
-            a.out_stride = self._heads("out", out, n, heads)
-        lse = None
-        if return_lse:
-            lse = torch.empty((n, heads), dtype=torch.float32, device=self.device)
-            a.lse = lse.data_ptr()
-        a.q, a.out, a.block_table, a.table_stride = q.data_ptr(), out.data_ptr(), block_table.data_ptr(), stride[0]
-        a.window, a.sinks = min(window, 1 << 62), min(sinks, 1 << 62)
-        a.batch, a.n_q_heads, a.table_width = n, heads, width
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
+            out_stride = self._heads("out", out, n, heads)
+        lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
         if n:
+            a = KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, q_stride, out_stride, block_table.data_ptr(),
+                         lens, stride[0], min(window, 1 << 62), min(sinks, 1 << 62), n, heads, width,
+                         self.head_dim ** -0.5 if scale is None else scale)
             self._call(self.lib.bam_launch_kv_attend, layout, C.byref(a))
         return (out, lse) if return_lse else out
