@@ -12,12 +12,12 @@ namespace bam {
 
 /* The flattened work list: sequence b has `n` chunks of CS tokens with something visible in them, in each of its
  * n_kv_heads * tiles units (a unit: 16 query heads of one key/value head), and the list is b-major, then unit, then
- * chunk.  A WARP is a worker: it takes one of as many equal runs as there are workers, copies their chunks into its own stages of shared memory
- * and keeps one running softmax.  Every warp reads the same amount whatever the lengths
- * are, a long sequence is split over many warps and a short one is not split at all (cuts that fall next to the edge
- * of a unit move there).  Warps share nothing and wait for nothing of one another until the end: one that does not
- * own a whole unit writes its running maximum, denominator and unnormalised sum to the scratch, and then the warps of
- * that unit wait for each other (they are co-resident, one cooperative launch) and each joins a part of the output,
+ * chunk.  A WARP is a worker: it takes one of as many equal runs as there are workers, copies their chunks into its own
+ * stages of shared memory and keeps one running softmax.  Every warp reads the same amount whatever the lengths are, a
+ * long sequence is split over many warps and a short one is not split at all (cuts that fall next to the edge of a unit
+ * move there).  Warps share nothing and wait for nothing of one another until the end: one that does not own a whole
+ * unit writes its running maximum, denominator and unnormalised sum to the scratch, and then the warps of that unit wait
+ * for each other (they are co-resident, one cooperative launch) and each joins a part of the output,
  * adding in a fixed order: the same bits on every run.
  *
  * What bounds it is reading keys and values once from HBM: 4 head_dim bytes a token for 4 head_dim flops a query head,
@@ -36,7 +36,7 @@ namespace bam {
 #define KV_MIN_CHUNKS 4u              /* a worker takes at least so many: below that splitting costs more than it saves */
 
 struct kv_seen_t {
-    int64_t len, first, begin;        /* visible: j < first, and begin <= j < len */
+    uint32_t len, first, begin;       /* visible: j < first, and begin <= j < len (lengths are 32-bit and positive) */
     uint32_t n_first, from, n;        /* chunks [0, n_first) and then [from, from + n - n_first) of the sequence */
 };
 
@@ -89,7 +89,7 @@ struct kv_shared_t {
     uint64_t warp_sum[KV_WORKERS + 1];
     uint32_t warp_max[KV_WORKERS + 1];
     volatile uint32_t abort;
-    struct { uint32_t b, u; uint64_t first; uint32_t n; } join[KV_WORKERS][2];
+    struct { uint32_t b, u, first, workers; } join[KV_WORKERS][2];      /* units to be joined, by whom */
 };
 
 BAM_DEV uint32_t ld_acquire_cta(const uint32_t* p) { uint32_t v; asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory"); return v; }
@@ -117,7 +117,7 @@ struct KvAttendWork {
     uint32_t piece;                                      /* tokens of a chunk that are sure to lie in one page: CS or 16 */
     float scale_log2;                                    /* its magnitude; the sign goes into the query */
     uint32_t q_sign;
-    int64_t window, sinks;
+    uint32_t window, sinks;                              /* 0x7fffffff at most */
     uint32_t* arrived;                                   /* per worker, all ones at the start: arrivals at the unit it begins */
     float* parts;                                        /* [worker][2]: rows x head_dim sums, 16 maxima, 16 denominators */
 
@@ -135,25 +135,26 @@ struct KvAttendWork {
     BAM_DEV kv_seen_t seen(uint32_t b, bool tell = false) const
     {
         kv_seen_t v;
-        v.len = __ldg(lens + b);
-        if (v.len < 0 || v.len > (int64_t)table_width * L.block_tokens) {
-            if (tell) L.bad_index((uint64_t)v.len);
+        const int32_t len = __ldg(lens + b);
+        v.len = (uint32_t)len;
+        if (len < 0 || v.len > (uint64_t)table_width * L.block_tokens) {
+            if (tell) L.bad_index((uint64_t)(int64_t)len);
             v.len = 0;
         }
         v.first = v.begin = v.len;
         if (window > 0 && window < v.len) {
-            const int64_t w0 = v.len - window;
+            const uint32_t w0 = v.len - window;
             v.first = sinks < v.len ? sinks : v.len;
             if (w0 > v.first) v.begin = w0; else v.first = v.begin = v.len;
         }
-        v.n_first = (uint32_t)((v.first + CS - 1) / CS);
-        v.from = (uint32_t)(v.begin / CS);
+        v.n_first = (v.first + CS - 1) / CS;
+        v.from = v.begin / CS;
         if (v.from < v.n_first) v.from = v.n_first;
-        const uint32_t end = (uint32_t)((v.len + CS - 1) / CS);
+        const uint32_t end = (v.len + CS - 1) / CS;
         v.n = v.n_first + (end > v.from ? end - v.from : 0u);
         return v;
     }
-    BAM_DEV static int64_t first_token(const kv_seen_t& v, uint32_t c) { return (int64_t)(c < v.n_first ? c : v.from + (c - v.n_first)) * CS; }
+    BAM_DEV static uint32_t first_token(const kv_seen_t& v, uint32_t c) { return (c < v.n_first ? c : v.from + (c - v.n_first)) * CS; }
 
     /* ---- the list ------------------------------------------------------------------------------------- */
     /* The list and the workers that share it: worker i takes the chunks from i * total / workers on (all differ by one
@@ -269,8 +270,8 @@ struct KvAttendWork {
                 while (pos >= (uint64_t)v.n * units && b + 1 < batch) { pos -= (uint64_t)v.n * units; v = seen(++b); }
                 if (v.n == 0) { sh.abort = 1; v.n = 1; }                                 /* the lengths changed under the launch */
                 const uint32_t u = (uint32_t)(pos / v.n), ci = (uint32_t)(pos - (uint64_t)u * v.n);
-                const int64_t t0 = first_token(v, ci), tb = t0 + k * piece;
-                int64_t lo = tb, hi = tb + piece < v.len ? tb + piece : v.len;
+                const uint32_t t0 = first_token(v, ci), tb = t0 + k * piece;
+                uint32_t lo = tb, hi = tb + piece < v.len ? tb + piece : v.len;
                 if (tb >= v.first && lo < v.begin) lo = v.begin;
                 if (tb + piece <= v.begin && hi > v.first) hi = v.first;
                 if (lo < hi) {
@@ -279,7 +280,7 @@ struct KvAttendWork {
                     else {
                         want = true;
                         page = L.page_of((uint64_t)block, u / tiles);
-                        rows = (uint32_t)(lo - t0) << 16 | (uint32_t)(hi - lo);
+                        rows = (lo - t0) << 16 | (hi - lo);
                         offset = (uint64_t)(lo % L.block_tokens) * row_bytes();
                     }
                 }
@@ -427,7 +428,7 @@ struct KvAttendWork {
      * parts, p = hi + lo, which keeps 16 (bf16) or more bits of them: the product runs twice, on a pipe that idles.
      * There is one copy of this code, for whole chunks and others: code that runs once a unit runs from a cold
      * instruction cache, at a microsecond for every few kilobytes. */
-    BAM_DEV void chunk(state_t& z, const uint32_t (&qa)[DMAX / 16][4], uint32_t stage, const kv_seen_t& v, int64_t t0) const
+    BAM_DEV void chunk(state_t& z, const uint32_t (&qa)[DMAX / 16][4], uint32_t stage, const kv_seen_t& v, uint32_t t0) const
     {
         const uint32_t lane = lane_id(), rb = row_bytes();
         const uint32_t x = pow2_row ? lane & 7u : ((lane & 7u) >> L.swz_shift) & L.swz_mask;
@@ -457,12 +458,12 @@ struct KvAttendWork {
              * weights are 0, and 0 x NaN is not 0 */
 #pragma unroll
             for (int i = 0; i < CS / 4; i++) {
-                const int64_t j = t0 + (i >> 1) * 8 + (lane & 3u) * 2 + (i & 1);
+                const uint32_t j = t0 + (i >> 1) * 8 + (lane & 3u) * 2 + (i & 1);
                 if (!((j < v.first || j >= v.begin) && j < v.len)) s[i >> 1][i & 1] = s[i >> 1][2 + (i & 1)] = -INFINITY;
             }
 #pragma unroll 1
             for (uint32_t i = lane; i < CS * (dim() / 8); i += 32) {
-                const int64_t j = t0 + i / (dim() / 8);
+                const uint32_t j = t0 + i / (dim() / 8);
                 if (!((j < v.first || j >= v.begin) && j < v.len))
                     asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(stage + CS * rb + i * 16u), "r"(0u) : "memory");
             }
@@ -642,7 +643,7 @@ struct KvAttendWork {
                 if (lane == 0) {
                     /* one release for the warp: what its other lanes wrote comes before it by the barrier */
                     red_add_release(arrived + i0, 1u);
-                    sh.join[w][n_join].b = b; sh.join[w][n_join].u = u; sh.join[w][n_join].first = U0; sh.join[w][n_join].n = v.n;
+                    sh.join[w][n_join].b = b; sh.join[w][n_join].u = u; sh.join[w][n_join].first = i0; sh.join[w][n_join].workers = cnt;
                 }
                 n_join++;
             }
@@ -662,15 +663,13 @@ struct KvAttendWork {
             return;
         }
         __syncwarp();
-        for (uint32_t k = 0; k < n_join; k++) join(sh, sh.join[w][k].b, sh.join[w][k].u, sh.join[w][k].first, sh.join[w][k].n, list, worker);
+        for (uint32_t k = 0; k < n_join; k++) join(sh.join[w][k].b, sh.join[w][k].u, sh.join[w][k].first, sh.join[w][k].workers, worker);
     }
 
     /* This worker's share of a unit that several worked on. */
-    BAM_DEV void join(kv_shared_t& sh, uint32_t b, uint32_t u, uint64_t U0, uint32_t n, const list_t& list, uint32_t worker) const
+    BAM_DEV void join(uint32_t b, uint32_t u, uint32_t i0, uint32_t cnt, uint32_t worker) const
     {
         const uint32_t lane = lane_id(), D = dim();
-        uint32_t i0, cnt;
-        workers_of(U0, U0 + n, list, i0, cnt);
         bam_status_t* st = L.r.cache.status;
         uint32_t polls = 0, gone = 0;
         uint64_t t0 = 0;
@@ -687,7 +686,7 @@ struct KvAttendWork {
         if (__shfl_sync(0xffffffffu, gone, 0)) return;
         const uint32_t h = u / tiles, r0 = (u - h * tiles) * KV_ROWS;
         const uint32_t rows = rows_of(u), quads = (rows + 7) / 8 * (D / 16) * 32, j = worker - i0;
-        const uint32_t g0 = (uint32_t)((uint64_t)quads * j / cnt), g1 = (uint32_t)((uint64_t)quads * (j + 1) / cnt);
+        const uint32_t g0 = quads * j / cnt, g1 = quads * (j + 1) / cnt;
         /* A quad is four elements of the output (see write_part); P lanes share one, each adds up to four parts of two quads
          * at a time, whose loads are all issued before the first is used: a part is one access to L2, and one after the
          * other they took 10 to 15 us of a call. */
@@ -877,7 +876,8 @@ static int launch_attend_nt(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     /* never 0: -infinity x 0, of a score that is not visible, would be NaN */
     w.scale_log2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, 1e-30f);
     w.q_sign = p->scale < 0.f ? 0x80008000u : 0u;
-    w.window = p->window; w.sinks = p->sinks;
+    w.window = p->window < 0x7fffffff ? (uint32_t)p->window : 0x7fffffffu;
+    w.sinks = p->sinks < 0x7fffffff ? (uint32_t)p->sinks : 0x7fffffffu;
     w.q32 = ((uintptr_t)p->q & 3) == 0 && p->q_stride[0] % 2 == 0 && p->q_stride[1] % 2 == 0;
     w.o32 = ((uintptr_t)p->out & 3) == 0 && p->out_stride[0] % 2 == 0 && p->out_stride[1] % 2 == 0;
     uint8_t* base = (uint8_t*)scratch;
