@@ -268,7 +268,12 @@ struct KvAttendWork {
             if (mine) {
                 kv_seen_t v = seen(b);
                 while (pos >= (uint64_t)v.n * units && b + 1 < batch) { pos -= (uint64_t)v.n * units; v = seen(++b); }
-                if (v.n == 0) { sh.abort = 1; v.n = 1; }                                 /* the lengths changed under the launch */
+                if (pos >= (uint64_t)v.n * units) {                                      /* the lengths changed under the launch */
+                    status_fail(L.r.cache.status, BAM_EINVAL, BAM_AT_RANGE, v.len);
+                    sh.abort = 1;
+                    v.n = 1;
+                    pos = 0;
+                }
                 const uint32_t u = (uint32_t)(pos / v.n), ci = (uint32_t)(pos - (uint64_t)u * v.n);
                 const uint32_t t0 = first_token(v, ci), tb = t0 + k * piece;
                 uint32_t lo = tb, hi = tb + piece < v.len ? tb + piece : v.len;
@@ -673,12 +678,14 @@ struct KvAttendWork {
         bam_status_t* st = L.r.cache.status;
         uint32_t polls = 0, gone = 0;
         uint64_t t0 = 0;
+        /* a warp whose pages are all in the cache may be done long before one whose pages come from the store: the limit is
+         * that of the launch */
         if (lane == 0) {
             while (ld_acquire_gpu(arrived + i0) != cnt - 1u && !gone) {
                 if (((++polls) & 63u) == 0u) {
                     const uint64_t now = global_timer_ns();
                     if (t0 == 0) t0 = now;
-                    if (now - t0 > st->spin_timeout_ns) status_fail(st, BAM_ETIMEDOUT, BAM_AT_KV_JOIN, i0);
+                    if (now - t0 > st->launch_timeout_ns) status_fail(st, BAM_ETIMEDOUT, BAM_AT_KV_JOIN, i0);
                     gone = status_bad(st) ? 1u : 0u;
                 }
             }
@@ -887,6 +894,7 @@ static int launch_attend_nt(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     w.piece = L.block_tokens % CS == 0 ? CS : 16;
     /* no more blocks than the longest sequences could keep busy */
     uint64_t chunks = ((uint64_t)p->table_width * L.block_tokens + CS - 1) / CS;
+    if (chunks > 0x80000000u / CS) chunks = 0x80000000u / CS;                             /* lengths are 32-bit numbers */
     if (p->window > 0) {
         const uint64_t seen = (uint64_t)p->window / CS + (uint64_t)(p->sinks < (1ll << 40) ? p->sinks : (1ll << 40)) / CS + 4;
         if (seen < chunks) chunks = seen;
