@@ -133,9 +133,9 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
         const bool failed = __any_sync(full, pending && slot == BAM_SLOT_ERR);
         const uint32_t m = __ballot_sync(full, got);
         if (m && !failed) rows(m, got ? L.r.get_cache_page_addr(slot) : 0);
-        if (write) __threadfence();
         __syncwarp();
-        /* one release per page: the lowest of the lanes that share it gives all their counts back */
+        /* one release per page: the lowest of the lanes that share it gives all their counts back (what the other lanes wrote
+         * comes before it by the barrier) */
         const uint32_t same = __match_any_sync(full, got ? slot : ~lane);
         if (got && lane == (uint32_t)(__ffs(same) - 1)) {
             /* rows that were read are in registers, or stored from there: there is nothing a release would have to wait for */
@@ -432,6 +432,9 @@ int kv_layout(bam_array* a, const bam_kv_layout_t* l, kv_layout_d_t* L)
 
 uint32_t lanes_of_row(uint32_t chunks) { uint32_t g = 1; while (g < chunks) g <<= 1; return g; }
 
+/* what a launch would fault on */
+bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+
 bool on_16(const void* p, int64_t s0, int64_t s1) { return ((uintptr_t)p & 15) == 0 && s0 % 8 == 0 && s1 % 8 == 0; }
 
 /* tokens a warp takes at a time: as many (up to `most`) as still make an item for every warp */
@@ -509,6 +512,8 @@ extern "C" int bam_launch_kv_append(bam_array_t a, const bam_kv_layout_t* layout
     int rc = kv_layout(a, layout, &L);
     if (rc) return rc;
     if (!p || !p->k || !p->v || !p->slots || p->n_tokens > 0x7fffffffull) return BAM_EINVAL;
+    if (!aligned(p->q, 2) || !aligned(p->k, 2) || !aligned(p->v, 2) || !aligned(p->q_out, 2) || !aligned(p->q_norm, 2) || !aligned(p->k_norm, 2) ||
+        !aligned(p->slots, 8) || !aligned(p->positions, 8) || !aligned(p->cos, 4) || !aligned(p->sin, 4)) return BAM_EINVAL;
     if (p->q && (!p->q_out || p->n_q_heads == 0 || p->n_q_heads > 65536)) return BAM_EINVAL;
     if (p->cos || p->sin) {
         if (!p->cos || !p->sin || !p->positions || p->n_positions == 0 || p->n_positions > 0x7fffffffffffull) return BAM_EINVAL;
@@ -551,6 +556,7 @@ extern "C" int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout
     int rc = kv_layout(a, layout, &L);
     if (rc) return rc;
     if (!slots_dev || !k_out_dev || !v_out_dev || !k_stride || !v_stride || n_tokens > 0x7fffffffull) return BAM_EINVAL;
+    if (!aligned(slots_dev, 8) || !aligned(k_out_dev, 2) || !aligned(v_out_dev, 2)) return BAM_EINVAL;
     rc = check_scratch(a, layout, scratch_dev, scratch_bytes);
     if (rc) return rc;
     if (n_tokens == 0) return BAM_OK;
@@ -568,6 +574,7 @@ extern "C" int bam_launch_kv_attend(bam_array_t a, const bam_kv_layout_t* layout
     int rc = kv_layout(a, layout, &L);
     if (rc) return rc;
     if (!p || !p->q || !p->out || !p->block_table || !p->seq_lens) return BAM_EINVAL;
+    if (!aligned(p->q, 2) || !aligned(p->out, 2) || !aligned(p->lse, 4) || !aligned(p->block_table, 4) || !aligned(p->seq_lens, 4)) return BAM_EINVAL;
     if (p->n_q_heads == 0 || p->n_q_heads > 65536 || p->n_q_heads % L.n_kv_heads) return BAM_EINVAL;
     if (p->batch > (1u << 20) || p->table_width == 0 || p->table_width > (1u << 27) || p->window < 0 || p->sinks < 0) return BAM_EINVAL;
     if (!std::isfinite(p->scale)) return BAM_EINVAL;

@@ -80,8 +80,8 @@ class KvCache:
         if t.dtype is self.dtype and shape == (n, heads, self.head_dim) and stride[2] == 1 and t.device == self.device:
             return stride[:2]
         self._on(name, t, self.dtype, 3)
-        if (n is not None and shape[0] != n) or shape[1] != heads or shape[2] != self.head_dim:
-            raise ValueError(f"{name} has shape {tuple(shape)}, wanted ({'n' if n is None else n}, {heads}, {self.head_dim})")
+        if shape != (n, heads, self.head_dim):
+            raise ValueError(f"{name} has shape {tuple(shape)}, wanted ({n}, {heads}, {self.head_dim})")
         if stride[2] != 1:
             raise ValueError(f"the elements of a head of {name} must be contiguous")
         return stride[:2]
@@ -139,7 +139,7 @@ class KvCache:
         if stream is not None:
             with self._on_stream(stream):
                 return self.append(k, v, slots, layer, positions, rope, rope_style, q, q_norm, k_norm, norm_eps, q_out)
-        n = k.shape[0]
+        n = k.shape[0] if k.dim() else 0
         k_stride, v_stride = self._heads("k", k, n, self.n_kv_heads), self._heads("v", v, n, self.n_kv_heads)
         at = self._flat("slots", slots, torch.int64, n)
         turn = 0, 0, 0, 0, 0, 0, 0                       # positions, cos, sin, rows, their stride, rotated elements, style
@@ -211,7 +211,7 @@ class KvCache:
         window > 0: only the last `window` tokens and the first `sinks` are visible; blocks without a visible token are
         not touched, their table entries may be anything.  scale defaults to head_dim ** -0.5.  Returns out, or
         (out, lse) with the logarithm of the softmax's denominator [batch, heads]; a sequence with nothing visible gets
-        zeros and -inf.  The new token's own key and value have to be appended first."""
+        zeros and -inf.  The new token's own key and value have to be appended first.  `out` may be q itself."""
         import torch
         if stream is not None:
             with self._on_stream(stream):

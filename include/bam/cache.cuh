@@ -16,8 +16,8 @@
  *    validate the slot's tag; eviction claims a slot with a 32-bit CAS that only succeeds on
  *    an unpinned, non-busy word, so a pinned page can never be recycled and a reader that
  *    raced with a recycle sees a tag mismatch, undoes its pin and looks the page up again.
- *  - Slots that were never used go out first; then eviction is a clock sweep over the slots (the reference's page_ticket hand, :1802), with up to 16 hands
- *    for a large cache: the SMs are dealt over the hands and every hand sweeps its own residue class of
+ *  - Slots that were never used go out first; then eviction is a clock sweep over the slots (the reference's
+ *    page_ticket hand, :1802), with up to 16 hands for a large cache: the SMs are dealt over the hands and every hand sweeps its own residue class of
  *    slots, so the misses of the whole GPU do not meet on one counter.
  *  - Read-only element accesses to resident pages take no pin at all: they validate a recycle
  *    generation around the data load (opt_probe / opt_validate below) and fall back to the pinning

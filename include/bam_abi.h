@@ -365,8 +365,9 @@ int bam_ctrl_write_store_from_device(bam_ctrl_t c, uint64_t byte_offset, const v
  * contiguous.  Every launch is asynchronous on `stream`, may be captured into a CUDA graph, and leaves the calling
  * thread's device as it was.  scratch_dev: bam_kv_scratch_bytes bytes of device memory, 128-byte aligned, set up once
  * by bam_kv_scratch_init.  Every launch leaves it ready for the next, also one that fails; launches that may run at the
- * same time need one each: one for every stream, one for every captured graph.  An index outside its range (a slot, position, block or length) is not followed: the status
- * block says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has finished, the rows that it concerns are undefined. */
+ * same time need one each: one for every stream, one for every captured graph.  An index outside its range (a slot,
+ * position, block or length) is not followed: the status block says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has
+ * finished, the rows that it concerns are undefined.  While the status block says anything, launches do nothing. */
 #define BAM_KV_BF16 0u
 #define BAM_KV_FP16 1u
 #define BAM_KV_ROPE_HALF 0u      /* pairs (i, i + rotary_dim / 2) */
@@ -380,7 +381,8 @@ uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* layout);
 int bam_kv_scratch_init(bam_array_t a, void* scratch_dev, uint64_t scratch_bytes, void* stream);
 
 /* Append: row t of k and v goes to slots[t] (int64; negative: the row is padding and nothing is written; slots are
- * distinct otherwise: of two rows for one slot neither is sure to be kept whole).  On the way each head of k, and of q where it is given, is
+ * distinct otherwise: of two rows for one slot neither is sure to be kept whole).  On the way each head of k, and of q
+ * where it is given, is
  *   normed:   y = x * rsqrt(mean(x^2) + norm_eps) * w      (q_norm / k_norm: head_dim elements of the layout's type, or NULL)
  *   rotated:  (a, b) -> (a c - b s, b c + a s) over the first rotary_dim (a multiple of 16) elements, with c and s the
  *             floats cos / sin[positions[t] * rope_stride + i] of pair i (cos NULL: no rotation; positions int64, below
@@ -410,7 +412,7 @@ int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t 
  * over the tokens j < seq_lens[b] (int32) that are visible: all of them, or with window > 0 the last `window` and the
  * first `sinks`.  Query head h reads key/value head h / (n_q_heads / n_kv_heads).  Token j of sequence b lies in block
  * block_table[b * table_stride + j / block_tokens] (int32); entries of blocks without a visible token are not read.
- * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL). */
+ * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL).  out may be q. */
 typedef struct {
     const void* q;
     void* out;

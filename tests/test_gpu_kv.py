@@ -463,7 +463,9 @@ def test_c_entries_refuse(cuda, bam):
     for c in (dict(k=None), dict(v=None), dict(slots=None), dict(n_tokens=1 << 31), dict(q=t.data_ptr()), dict(scratch=None), dict(scratch=sp + 64),
               dict(size=sb - 1), dict(rope, sin=None), dict(rope, positions=None), dict(rope, n_positions=0), dict(rope, rotary_dim=24),
               dict(rope, rotary_dim=80), dict(rope, rope_stride=-1), dict(rope, rope_style=2), dict(k_norm=t.data_ptr(), norm_eps=-1.0),
-              dict(k_norm=t.data_ptr(), norm_eps=float("nan")), dict(q=t.data_ptr(), q_out=t.data_ptr(), n_q_heads=0)):
+              dict(k_norm=t.data_ptr(), norm_eps=float("nan")), dict(q=t.data_ptr(), q_out=t.data_ptr(), n_q_heads=0),
+              dict(k=t.data_ptr() + 1), dict(v=t.data_ptr() + 1), dict(slots=i64.data_ptr() + 4), dict(rope, cos=f.data_ptr() + 2),
+              dict(rope, positions=i64.data_ptr() + 4), dict(q=t.data_ptr(), q_out=t.data_ptr() + 1, n_q_heads=2)):
         assert append(**c) == EINVAL, c
     at = dict(q=t.data_ptr(), out=t.data_ptr(), q_stride=(128, 64), out_stride=(128, 64), block_table=i32.data_ptr(), seq_lens=i32.data_ptr(),
               table_stride=1, batch=1, n_q_heads=2, table_width=1, scale=0.1)
@@ -478,8 +480,12 @@ def test_c_entries_refuse(cuda, bam):
         return lib.bam_launch_kv_attend(h, L(), C.byref(a), scratch, size, None)
     assert attend() == 0 and attend(batch=0) == 0
     for c in (dict(q=None), dict(out=None), dict(block_table=None), dict(seq_lens=None), dict(n_q_heads=3), dict(n_q_heads=0), dict(table_width=0),
-              dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=(1 << 20) + 1), dict(size=0), dict(scratch=None)):
+              dict(window=-1), dict(sinks=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(batch=(1 << 20) + 1), dict(size=0), dict(scratch=None),
+              dict(q=t.data_ptr() + 1), dict(out=t.data_ptr() + 1), dict(lse=f.data_ptr() + 2), dict(block_table=i32.data_ptr() + 2),
+              dict(seq_lens=i32.data_ptr() + 2)):
         assert attend(**c) == EINVAL, c
+    for c in ((i64.data_ptr() + 4, t.data_ptr(), t.data_ptr()), (i64.data_ptr(), t.data_ptr() + 1, t.data_ptr()), (i64.data_ptr(), t.data_ptr(), t.data_ptr() + 1)):
+        assert lib.bam_launch_kv_gather(h, L(), 1, *c, two, two, sp, sb, None) == EINVAL
     # an array that starts inside a page is refused
     a2 = bam.Array.from_ranges(kv.cache, 512, [(0, 512, 0, 64)])
     assert lib.bam_kv_scratch_bytes(a2.h, L(n_blocks=1, n_kv_heads=1)) == 0
@@ -749,4 +755,26 @@ def test_offsets_beyond_32_bits(cuda, bam):
     out = kv.attend(q, table, torch.ones(3, dtype=torch.int32, device="cuda"))
     assert torch.equal(out, v[table[:, 0].long()].expand(3, 2, D))     # one visible token: its value
     assert kv.cache.ctrl.status() == (0, "none", 0)
+    done(kv)
+
+
+def test_attend_in_place_and_slots_that_repeat(cuda, bam):
+    """`out` is q: the warps that share a sequence write its rows when all of them have read q.  A slot may be gathered
+    more than once."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(15)
+    lens = [3000, 5, 0, 700]
+    kv = make(bam, torch, 240, 2, 64, torch.bfloat16, page=4096)
+    k, v, table = fill(torch, g, kv, lens)
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for width in (64, 67):                                       # rows that share 32-byte sectors, too
+        q = torch.zeros(4, 24, width, dtype=torch.bfloat16, device="cuda")[..., width - 64:]
+        q.copy_(rand(torch, g, 4, 24, 64, dtype=torch.bfloat16, scale=2.0))
+        want = kv.attend(q, table, ls)
+        assert kv.attend(q, table, ls, out=q) is q
+        assert torch.equal(q, want)
+    slots = torch.randint(0, 40, (500,), generator=g, device="cuda")
+    bk, bv = kv.gather(slots)
+    assert torch.equal(bk, k[slots]) and torch.equal(bv, v[slots])
     done(kv)
