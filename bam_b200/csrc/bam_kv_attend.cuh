@@ -13,9 +13,8 @@ namespace bam {
 /* The flattened work list: sequence b has `n` chunks of CS tokens with something visible in them, in each of its
  * n_kv_heads * tiles units (a unit: 16 query heads of one key/value head), and the list is b-major, then unit, then
  * chunk.  A WARP is a worker: it takes one of as many equal runs as there are workers, copies their chunks into its own
- * stages of shared memory and keeps one running softmax.  Every warp reads the same amount whatever the lengths are, a
- * long sequence is split over many warps and a short one is not split at all (cuts that fall next to the edge of a unit
- * move there).  Warps share nothing and wait for nothing of one another until the end: one that does not own a whole
+ * stages of shared memory and keeps one running softmax.  Every warp reads the same amount whatever the lengths are: a
+ * long sequence is split over many warps, short ones are as many to a warp.  Warps share nothing and wait for nothing of one another until the end: one that does not own a whole
  * unit writes its running maximum, denominator and unnormalised sum to the scratch, and then the warps of that unit wait
  * for each other (they are co-resident, one cooperative launch) and each joins a part of the output,
  * adding in a fixed order: the same bits on every run.
@@ -158,12 +157,12 @@ struct KvAttendWork {
 
     /* ---- the list ------------------------------------------------------------------------------------- */
     /* The list and the workers that share it: worker i takes the chunks from i * total / workers on (all differ by one
-     * chunk at most), but a cut that falls within `slack` chunks of the edge of a unit moves there: a join costs what
-     * two chunks do. */
+     * chunk at most).  Cuts that moved to the edge of a unit nearby saved joins and no time: 168 us both ways at 64
+     * sequences of 2500-4100 tokens. */
     struct list_t {
-        uint64_t total, workers, slack;
+        uint64_t total, workers;
         BAM_DEV uint64_t cut(uint64_t i) const { return i * total / workers; }
-        BAM_DEV uint64_t worker_of(uint64_t x) const { return ((x + 1) * workers - 1) / total; }      /* before cuts move */
+        BAM_DEV uint64_t worker_of(uint64_t x) const { return ((x + 1) * workers - 1) / total; }
     };
 
     /* Where worker i's run begins.  All lanes. */
@@ -198,22 +197,16 @@ struct KvAttendWork {
             at += __shfl_sync(0xffffffffu, upto - span, src);
             break;
         }
-        const uint64_t n = seen(p.b).n, in = (x - at) % n;
         p.f = x;
-        if (in <= list.slack) p.f = x - in;
-        else if (n - in <= list.slack) p.f = x + (n - in);
-        p.pos = p.f - at;
+        p.pos = x - at;
         return p;
     }
     /* the first worker of the unit [U0, U1), and how many there are */
     BAM_DEV static void workers_of(uint64_t U0, uint64_t U1, const list_t& list, uint32_t& first, uint32_t& count)
     {
-        uint64_t i0 = list.worker_of(U0), i1 = list.worker_of(U1 - 1);
-        const uint64_t up = list.cut(i0 + 1), down = list.cut(i1);
-        if (up < U1 && up - U0 <= list.slack) i0++;
-        if (down > U0 && down - U0 > list.slack && U1 - down <= list.slack) i1--;
+        const uint64_t i0 = list.worker_of(U0);
         first = (uint32_t)i0;
-        count = (uint32_t)(i1 - i0 + 1);
+        count = (uint32_t)(list.worker_of(U1 - 1) - i0 + 1);
     }
 
     /* ---- pages and copies ----------------------------------------------------------------------------- */
@@ -834,9 +827,8 @@ struct KvAttendWork {
         sh.before[t] = before * units;
         /* workers: all there are, but none of them with less than KV_MIN_CHUNKS (or the longest unit, if that is shorter) */
         const uint64_t n_workers = (uint64_t)nvb * KV_WORKERS, least = longest < KV_MIN_CHUNKS ? longest : KV_MIN_CHUNKS;
-        list_t list = { total, total >= n_workers * least ? n_workers : total / (least ? least : 1u), 0 };
+        list_t list = { total, total >= n_workers * least ? n_workers : total / (least ? least : 1u) };
         if (list.workers == 0) list.workers = 1;
-        list.slack = total / list.workers / 8 < 2 ? total / list.workers / 8 : 2;
         /* sequences with nothing visible */
         for (uint32_t b = vb; b < batch; b += nvb) {
             if (seen(b).n == 0) {
@@ -851,10 +843,8 @@ struct KvAttendWork {
         /* neighbours in the list on different SMs: the workers of a short list spread out */
         const uint32_t worker = w * nvb + vb;
         if (w < KV_WORKERS) {
-            kv_place_t from = { 0, 0, 0 }, to = from;
-#pragma unroll 1
-            for (uint32_t k = 0; k < 2; k++) { from = to; to = begin_of(sh, worker + (uint64_t)k, list); }
-            if (lane == 0) { sh.from[w] = from; sh.chunks[w] = (uint32_t)(to.f - from.f); }
+            const kv_place_t from = begin_of(sh, worker, list);
+            if (lane == 0) { sh.from[w] = from; sh.chunks[w] = from.f < total ? (uint32_t)(list.cut(worker + 1ull) - from.f) : 0u; }
         }
         __syncthreads();
         if (w < KV_WORKERS) {
