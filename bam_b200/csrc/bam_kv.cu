@@ -156,8 +156,6 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
  * with room for all.)  Items differ in length, hence the drawing; which warp writes a row changes nothing in it.
  * Bytes bound it, every row is read and written once; what that needs is rows in flight: several rows of a lane are loaded
  * before the first is worked on.  Angles are loaded once per token and item for the queries. */
-#define KV_Q_HEADS 16u
-#define KV_K_HEADS 2u
 #define KV_ROWS_AHEAD 4
 
 /* VEC: every row, weight and angle lies on a 16-byte boundary. */
@@ -170,7 +168,7 @@ struct KvAppendWork {
     uint16_t* q_out;
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, qo_st, qo_sh;      /* element strides of token and head */
     uint64_t n_tokens;
-    uint32_t n_q_heads, lanes_per_row, k_tokens, q_tokens, k_parts, q_parts;
+    uint32_t n_q_heads, lanes_per_row, k_tokens, q_tokens, k_heads, q_heads, k_parts, q_parts;
     const int64_t* slots;
     kv_rope_d_t rope;
     const uint16_t *q_norm, *k_norm;
@@ -294,7 +292,7 @@ struct KvAppendWork {
                 for (int i = 0; i < 8; i++) { const float2 f = kv_type<T>::unpack(w[i]); ln.w[2 * i] = f.x; ln.w[2 * i + 1] = f.y; }
             }
             if (queries_of) {
-                const uint32_t h0 = part * KV_Q_HEADS, n = n_q_heads - h0 < KV_Q_HEADS ? n_q_heads - h0 : KV_Q_HEADS;
+                const uint32_t h0 = part * q_heads, n = n_q_heads - h0 < q_heads ? n_q_heads - h0 : q_heads;
                 const int64_t pos = lane < nt ? position(t0 + lane, slots[t0 + lane] < 0) : 0;
                 for (uint32_t i = 0; i < nt; i++) {
                     const int64_t p = __shfl_sync(full, pos, i);
@@ -318,7 +316,7 @@ struct KvAppendWork {
                     const int64_t pos = live ? position(t, false) : 0;
                     const uint32_t row = live ? (uint32_t)((uint64_t)slots[t] % L.block_tokens) : 0;
                     const uint32_t run = in_run & __ballot_sync(full, pos >= 0);
-                    const uint32_t h0 = part * KV_K_HEADS, nh = L.n_kv_heads - h0 < KV_K_HEADS ? L.n_kv_heads - h0 : KV_K_HEADS;
+                    const uint32_t h0 = part * k_heads, nh = L.n_kv_heads - h0 < k_heads ? L.n_kv_heads - h0 : k_heads;
                     if (run && !kv_with_pages(L, lane < nh, L.page_of(at, h0 + lane), true, (uint32_t)warp, [&](uint32_t m, uint64_t addr) {
                             keys(t1, run, 32u - __clz(run), h0, nh, m, addr, row, pos, ln, j, G, grp);
                         })) return;
@@ -445,6 +443,14 @@ uint32_t tokens_of_item(uint64_t n_tokens, uint32_t parts, uint64_t warps, uint3
     return t;
 }
 
+/* heads a warp takes at a time: as many (`least` to `most`) as still make `enough` items of so many pieces */
+uint32_t heads_of_item(uint32_t heads, uint64_t pieces, uint64_t enough, uint32_t most, uint32_t least)
+{
+    uint32_t h = most;
+    while (h > least && pieces * ((heads + h - 1) / h) < enough) h >>= 1;
+    return h;
+}
+
 }  // namespace
 
 extern "C" uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* layout)
@@ -483,9 +489,11 @@ static int launch_append_as(bam_array_t a, const kv_layout_d_t& L, const bam_kv_
     w.v_st = p->v_stride[0]; w.v_sh = p->v_stride[1]; w.qo_st = p->q_out_stride[0]; w.qo_sh = p->q_out_stride[1];
     w.n_tokens = p->n_tokens; w.n_q_heads = p->q ? p->n_q_heads : 0;
     w.lanes_per_row = lanes_of_row(L.chunks / 2);
-    w.k_parts = (L.n_kv_heads + KV_K_HEADS - 1) / KV_K_HEADS;
-    w.q_parts = (w.n_q_heads + KV_Q_HEADS - 1) / KV_Q_HEADS;
     const uint64_t warps = (uint64_t)a->pc->ctrl->num_sms * w.min_blocks * (w.threads / 32);
+    w.k_heads = heads_of_item(L.n_kv_heads, p->n_tokens / L.block_tokens, warps / 4, 4, 1);
+    w.q_heads = heads_of_item(w.n_q_heads, p->n_tokens, 2 * warps, 32, 16);
+    w.k_parts = (L.n_kv_heads + w.k_heads - 1) / w.k_heads;
+    w.q_parts = (w.n_q_heads + w.q_heads - 1) / w.q_heads;
     w.k_tokens = tokens_of_item(p->n_tokens, w.k_parts, warps, 32);
     w.q_tokens = tokens_of_item(p->n_tokens, w.q_parts, 2 * warps, 16);
     w.slots = p->slots;
