@@ -149,13 +149,19 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
     return true;
 }
 
-/* The work is cut into items that warps draw in turn: first KV_K_HEADS of the key/value heads of the runs that begin in k_tokens
- * consecutive tokens, then KV_Q_HEADS of the query heads of q_tokens tokens.  A run is the tokens in a row that go to one
+/* The work is cut into items that warps draw in turn: first k_heads of the key/value heads of the runs that begin in k_tokens
+ * consecutive tokens, then q_heads of the query heads of q_tokens tokens.  A run is the tokens in a row that go to one
  * block: one warp writes its share of it, to the end of the run and not of the item, and pins each page once.  (Warps that
  * miss the same page at once claim a slot each: a prompt whose pages were written by two warps each evicted half of a cache
  * with room for all.)  Items differ in length, hence the drawing; which warp writes a row changes nothing in it.
- * Bytes bound it, every row is read and written once; what that needs is rows in flight: several rows of a lane are loaded
- * before the first is worked on.  Angles are loaded once per token and item for the queries. */
+ * Items are as large as still makes enough of them: a warp pins its pages together and loads angles and weights once an
+ * item.  16000 tokens of 32 + 8 heads of 128, gathered again: 144 us with items of 32 and 4 heads, 152 with 16 and 1, 170 with
+ * 8 query heads (which are too few rows in flight); 777 tokens of 15 + 3 heads of 256: 33 us with 1 key/value head, 37 with
+ * 2, 41 with 4.
+ * Bytes bound it, every row is read and written once; what that needs is rows in flight: four rows of a lane are loaded before
+ * the first is worked on (two: 164 us instead of 150).  It reaches 3.5 TB/s, 0.53 of a copy (111 us for 393 MB without the
+ * gather): 16 warps an SM, all that 128 registers allow, wait for their loads in turn and issue in 40 % of the cycles;
+ * a second row of keys in flight spilled (190 us). */
 #define KV_ROWS_AHEAD 4
 
 /* VEC: every row, weight and angle lies on a 16-byte boundary. */
@@ -331,6 +337,11 @@ struct KvAppendWork {
 /* gather                                                                                  */
 /* ====================================================================================== */
 
+/* Items of up to 32 tokens of one head, drawn in turn: a lane looks up the page of a token, then groups of lanes copy rows.
+ * Bytes bound it.  30001 tokens of 8 heads of 128 take 54 us, 4.6 TB/s: about 12 us of a launch that starts, looks its first
+ * pages up and ends, and the rest at what a copy reaches.  Three blocks an SM, four rows of a lane loaded before the first
+ * is stored (two: 65 us; eight at two blocks: 71).  Through shared memory with bulk copies, the look-ups of an item wait for
+ * its one stage: 64 to 73 us. */
 template <bool VEC>
 struct KvGatherWork {
     static constexpr int threads = BAM_THREADS, min_blocks = 3;
@@ -364,8 +375,6 @@ struct KvGatherWork {
             }
             const uint32_t row = slot >= 0 ? (uint32_t)((uint64_t)slot % L.block_tokens) : 0;
             const uint64_t page = slot >= 0 ? L.page_of((uint64_t)slot / L.block_tokens, h) : 0;
-            /* KV_ROWS_AHEAD rows of a lane are loaded before the first is stored: bytes bound this, if enough of them are
-             * under way */
             auto copy = [&](uint32_t m, uint64_t addr) {
                 for (uint32_t i0 = 0; i0 < tokens_per_item; i0 += rows * KV_ROWS_AHEAD) {
                     uint4 kk[KV_ROWS_AHEAD], vv[KV_ROWS_AHEAD];
@@ -494,7 +503,7 @@ static int launch_append_as(bam_array_t a, const kv_layout_d_t& L, const bam_kv_
     w.q_heads = heads_of_item(w.n_q_heads, p->n_tokens, 2 * warps, 32, 16);
     w.k_parts = (L.n_kv_heads + w.k_heads - 1) / w.k_heads;
     w.q_parts = (w.n_q_heads + w.q_heads - 1) / w.q_heads;
-    w.k_tokens = tokens_of_item(p->n_tokens, w.k_parts, warps, 32);
+    w.k_tokens = tokens_of_item(p->n_tokens, w.k_parts, warps, KV_MAX_LANE_TOKENS);
     w.q_tokens = tokens_of_item(p->n_tokens, w.q_parts, 2 * warps, 16);
     w.slots = p->slots;
     w.rope.positions = p->positions; w.rope.cos = p->cos; w.rope.sin = p->sin; w.rope.n_positions = p->n_positions;
