@@ -161,7 +161,8 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
  * Bytes bound it, every row is read and written once; what that needs is rows in flight: four rows of a lane are loaded before
  * the first is worked on (two: 164 us instead of 150).  It reaches 3.5 TB/s, 0.53 of a copy (111 us for 393 MB without the
  * gather): 16 warps an SM, all that 128 registers allow, wait for their loads in turn and issue in 40 % of the cycles;
- * a second row of keys in flight spilled (190 us). */
+ * a second row of keys in flight spilled (190 us), rows prefetched through shared memory, 96 KB a block, took 156 us instead
+ * of 142. */
 #define KV_ROWS_AHEAD 4
 
 /* VEC: every row, weight and angle lies on a 16-byte boundary. */
