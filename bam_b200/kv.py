@@ -41,6 +41,8 @@ class KvCache:
             raise ValueError(f"head_dim must be a multiple of 16 up to 256, not {head_dim}")
         if n_blocks < 1 or n_kv_heads < 1 or n_layers < 1:
             raise ValueError("n_blocks, n_kv_heads and n_layers must be positive")
+        if n_blocks > 0x7fffffff or n_kv_heads > 65536:
+            raise ValueError("at most 2^31 - 1 blocks and 65536 heads")
         row = 4 * head_dim                                       # a key and a value
         if block_tokens is None:
             block_tokens = cache.page_size // row // 16 * 16

@@ -557,7 +557,7 @@ def test_captured_graphs(cuda, bam):
 
 
 def test_two_streams_and_caches_at_once(cuda, bam):
-    """Calls that run at the same time: two streams on one cache, and a second cache over the same controller."""
+    """Calls that run at the same time: two streams on one cache."""
     torch = cuda
     g = torch.Generator(device="cuda").manual_seed(9)
     lens = [800, 30, 400]
@@ -778,3 +778,48 @@ def test_attend_in_place_and_slots_that_repeat(cuda, bam):
     bk, bv = kv.gather(slots)
     assert torch.equal(bk, k[slots]) and torch.equal(bv, v[slots])
     done(kv)
+
+
+def test_launches_that_fetch_at_once(cuda, bam):
+    """Attention over one cache and a gather from a second one, both with more pages than slots, and a page scan through a
+    third, on three streams over one controller: each launch's controller blocks serve the others' commands, too."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(16)
+    lens, page, blocks = [1500, 700, 900], 4096, 200
+    c = bam.Controller(blocks * 4 * page, 0, queue_depth=64, num_queues=16)
+    c.configure(ctrl_blocks=2, spin_timeout_ns=5 * SEC)
+    c.set_launch_timeout(30 * SEC)
+    c.set_max_grid(24)
+    caches = [bam.PageCache(c, page, slots) for slots in (150, 150, 2 * blocks + 8)]
+    kvs = [bam.KvCache(caches[i], blocks, 2, 64, store_byte_offset=i * blocks * 2 * page) for i in range(2)]
+    k, v, table = fill(torch, g, kvs[0], lens)
+    every = torch.arange(len(k), device="cuda")
+    kvs[0].append(k, v, every)
+    kvs[1].append(v, k, every)
+    for cache in caches:
+        cache.flush()
+    scanned = bam.Array(caches[2], blocks * 2 * page // 8)
+    assert c.status() == (0, "none", 0)
+    words = int(torch.from_numpy(c.store_numpy("int64")[:blocks * 2 * page // 8].copy()).sum())
+    q = rand(torch, g, 3, 8, 64, dtype=torch.bfloat16, scale=2.0)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = attend64(torch, q, k, v, table, lens, kvs[0].block_tokens, 0.125)
+    order = [torch.randperm(len(k), generator=g, device="cuda") for _ in range(4)]
+    sums = torch.zeros(4, dtype=torch.int64, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs, rows = [], []
+    for i in range(4):
+        outs.append(kvs[0].attend(q, table, ls, stream=streams[0]))
+        rows.append(kvs[1].gather(order[i], stream=streams[1]))
+        scanned.page_scan(blocks * 2, sums[i:], stream=streams[2].cuda_stream)
+    torch.cuda.synchronize()
+    assert c.status() == (0, "none", 0)
+    for i in range(4):
+        check_attend(torch, outs[i], None, ref, torch.bfloat16)
+        assert torch.equal(rows[i][0], v[order[i]]) and torch.equal(rows[i][1], k[order[i]])
+        assert int(sums[i]) == words
+    for x, cache in zip((*kvs, scanned), caches):
+        assert cache.audit() == 0
+        x.close(); cache.close()
+    c.close()

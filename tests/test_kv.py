@@ -57,7 +57,7 @@ def test_refuses_types_and_counts(bam):
     import torch
     with pytest.raises(ValueError):
         bam.KvCache(_Pages(8192), 4, 2, 64, dtype=torch.float32)
-    for blocks, heads, layers in ((0, 1, 1), (1, 0, 1), (1, 1, 0)):
+    for blocks, heads, layers in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1 << 31, 1, 1), (1, 65537, 1)):
         with pytest.raises(ValueError):
             bam.KvCache(_Pages(8192), blocks, heads, 64, n_layers=layers)
 
