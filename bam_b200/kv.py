@@ -29,7 +29,11 @@ class KvCache:
 
     One page of `cache` holds the keys and the values of one block for one head; block_tokens defaults to what fits (a
     multiple of 16).  A token's slot is block * block_tokens + its place in the block.  `dist` lays the pages over the
-    controllers of the cache (REPLICATE or STRIPE), store_byte_offset places them in the store."""
+    controllers of the cache (REPLICATE or STRIPE), store_byte_offset places them in the store.
+
+    The calls run on the current stream of the cache's device or on `stream` (a torch stream or a raw handle), in whose
+    memory pool their results are; the order between streams, and that tensors live long enough, is the caller's affair as
+    for any work on another stream.  They may be captured into CUDA graphs.  Results carry no gradient."""
 
     def __init__(self, cache, n_blocks, n_kv_heads, head_dim, dtype=None, block_tokens=None, n_layers=1, store_byte_offset=0,
                  dist=REPLICATE):
