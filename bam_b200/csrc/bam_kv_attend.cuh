@@ -12,23 +12,24 @@ namespace bam {
 
 /* The flattened work list: sequence b has `n` chunks of CS tokens with something visible in them, in each of its
  * n_kv_heads * tiles units (a unit: 16 query heads of one key/value head), and the list is b-major, then unit, then
- * chunk.  A WARP is a worker: it takes one of as many equal runs as there are workers, copies their chunks into its own
- * stages of shared memory and keeps one running softmax.  Every warp reads the same amount whatever the lengths are: a
- * long sequence is split over many warps, short ones are as many to a warp.  Warps share nothing and wait for nothing of one another until the end: one that does not own a whole
- * unit writes its running maximum, denominator and unnormalised sum to the scratch, and then the warps of that unit wait
- * for each other (they are co-resident, one cooperative launch) and each joins a part of the output,
- * adding in a fixed order: the same bits on every run.
+ * chunk.  A WARP is a worker: it takes one of as many equal runs as there are workers, copies their chunks into its
+ * own stages of shared memory and keeps one running softmax.  Every warp reads the same amount whatever the lengths
+ * are: a long sequence is split over many warps, short ones are as many to a warp.  Warps share nothing and wait for
+ * nothing of one another until the end: one that does not own a whole unit writes its running maximum, denominator and
+ * unnormalised sum to the scratch, and then the warps of that unit wait for each other (they are co-resident, one
+ * cooperative launch) and each joins a part of the output, adding in a fixed order: the same bits on every run.
  *
  * What bounds it is reading keys and values once from HBM: 4 head_dim bytes a token for 4 head_dim flops a query head,
- * 8 flops a byte at 8 query heads.  So the design feeds bulk copies: three worker warps a block, two blocks an SM, two or
- * more chunks under way for each (200 KB of an SM's shared memory).  The fourth warp of a block looks their pages up and
- * pins them up to 16 chunks ahead: a look-up is three dependent accesses that miss L2 while the rows stream through it,
- * 2 to 5 us (done by the workers themselves, 32 pages at a time, it cost 3 us of 186, and registers that wide heads lack).
- * The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured): up to 16 query heads are
- * all there is, the 128-row tcgen05 tiles would be seven eighths padding.  The scores have the queries as rows and the sums
- * as columns, S = Q K^T and O^T = V^T P^T: the scores are then where the second product wants its right operand, and
- * eight query heads take half of the instructions (and of the registers for O) that sixteen do.  At 128 dimensions a
- * chunk of 32 tokens takes 64 of them, 130 of the 710 cycles that HBM needs to deliver it to an SM.
+ * 8 flops a byte at 8 query heads.  So the design feeds bulk copies: three worker warps a block, two blocks an SM, two
+ * or more chunks under way for each (200 KB of an SM's shared memory).  The fourth warp of a block looks their pages
+ * up and pins them up to 16 chunks ahead: a look-up is three dependent accesses that miss L2 while the rows stream
+ * through it, 2 to 5 us (done by the workers themselves, 32 pages at a time, it cost 3 us of 186, and registers that
+ * wide heads lack).  The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured):
+ * up to 16 query heads are all there is, tcgen05 tiles of 64 or 128 rows would be mostly padding.  The scores have
+ * the queries as rows and the sums as columns, S = Q K^T and O^T = V^T P^T: the scores are then where the second
+ * product wants its right operand, and eight query heads take half of the instructions (and of the registers for O)
+ * that sixteen do.  At 128 dimensions a chunk of 32 tokens takes 64 of them, 130 of the 710 cycles that HBM needs to
+ * deliver it to an SM.
  *
  * Measured (bf16, 8 key/value heads of 128): 64 sequences of 2500 to 4100 tokens, 867 MB, 163 us = 5.3 TB/s, 0.81 of a copy
  * (6.7 TB/s between the first chunk and the last); 32 of 130 to 1700, 120 MB, 47 us.  What the short ones wait for: 3 us until
