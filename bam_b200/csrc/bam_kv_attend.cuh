@@ -4,6 +4,7 @@
 #ifndef BAM_KV_ATTEND_CUH
 #define BAM_KV_ATTEND_CUH
 
+#include <cfloat>
 #include <cstring>
 
 #include "bam_kv.cuh"
@@ -121,7 +122,7 @@ struct KvAttendWork {
     uint32_t group, tiles;                               /* query heads of a key/value head, units they make */
     uint32_t ahead;                                      /* KV_AHEAD, or less in a small cache */
     uint32_t piece;                                      /* tokens of a chunk that are sure to lie in one page: CS or 16 */
-    float scale_log2;                                    /* its magnitude; the sign goes into the query */
+    float scale_log2;                                    /* the scale's magnitude x log2(e); its sign goes into the query */
     uint32_t q_sign;
     uint32_t window, sinks;                              /* 0x7fffffff at most */
     uint32_t* arrived;                                   /* per worker, all ones at the start: arrivals at the unit it begins */
@@ -418,6 +419,8 @@ struct KvAttendWork {
         float o[NT][DMAX / 16][4];
         float m[2], l[2];
     };
+    /* a score's weight beside a maximum, both unscaled */
+    BAM_DEV float weight_of(float s, float m) const { return exp2_fast((s - m) * scale_log2); }
     /* what a thread knows of queries lane / 4 and lane / 4 + 8, for the queries of its columns */
     BAM_DEV static void to_columns(float x0, float x1, float (&c)[NT][2])
     {
@@ -429,7 +432,9 @@ struct KvAttendWork {
         }
     }
 
-    /* One chunk: S = Q K^T, p = 2^(S scale log2(e) - m), O^T += V^T p^T.  The weights go into the product as two 16-bit
+    /* One chunk: S = Q K^T, p = 2^((S - m) scale log2(e)), O^T += V^T p^T.  m is a maximum of S as it is, and the difference
+     * comes before the scale: the largest weight is 1 however large the scores are.  (With a scaled m it would be 2 to the
+     * rounding of m, anything beyond 2^24.)  The weights go into the product as two 16-bit
      * parts, p = hi + lo, which keeps 16 (bf16) or more bits of them: the product runs twice, on a pipe that idles.
      * There is one copy of this code, for whole chunks and others: code that runs once a unit runs from a cold
      * instruction cache, at a microsecond for every few kilobytes. */
@@ -484,10 +489,10 @@ struct KvAttendWork {
         }
         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-        const float n0 = fmaxf(z.m[0], mx0 * scale_log2), n1 = fmaxf(z.m[1], mx1 * scale_log2);
+        const float n0 = fmaxf(z.m[0], mx0), n1 = fmaxf(z.m[1], mx1);
         const float c0 = n0 == -INFINITY ? 0.f : n0, c1 = n1 == -INFINITY ? 0.f : n1;     /* nothing seen yet: exp2(-inf - 0) = 0 */
         if (__any_sync(0xffffffffu, n0 != z.m[0] || n1 != z.m[1])) {
-            const float a0 = exp2_fast(z.m[0] - c0), a1 = exp2_fast(z.m[1] - c1);
+            const float a0 = weight_of(z.m[0], c0), a1 = weight_of(z.m[1], c1);
             float a[NT][2];
             to_columns(a0, a1, a);
             z.l[0] *= a0; z.l[1] *= a1;
@@ -505,7 +510,7 @@ struct KvAttendWork {
             for (int n = 0; n < NT; n++) {
                 float p[2];
 #pragma unroll
-                for (int e = 0; e < 2; e++) p[e] = exp2_fast(fmaf(s[i][2 * n + e], scale_log2, n ? -c1 : -c0));
+                for (int e = 0; e < 2; e++) p[e] = weight_of(s[i][2 * n + e], n ? c1 : c0);
                 z.l[n] += p[0] + p[1];
                 hi[n][i] = kv_type<T>::pack(p[0], p[1]);
                 const float2 h = kv_type<T>::unpack(hi[n][i]);
@@ -534,7 +539,7 @@ struct KvAttendWork {
         if (o32) *reinterpret_cast<uint32_t*>(p) = w;
         else { p[0] = (uint16_t)w; p[1] = (uint16_t)(w >> 16); }
     }
-    BAM_DEV static float lse_of(float m, float l) { return m == -INFINITY ? -INFINITY : m * 0.69314718055994531f + logf(l); }
+    BAM_DEV float lse_of(float m, float l) const { return m == -INFINITY ? -INFINITY : m * scale_log2 * 0.69314718055994531f + logf(l); }
 
     /* the unit's result from one warp's registers */
     BAM_DEV void write_out(const state_t& z, uint32_t b, uint32_t u) const
@@ -738,12 +743,12 @@ struct KvAttendWork {
                         float m = M[e][c2];
 #pragma unroll
                         for (int k = 0; k < 4; k++) m = fmaxf(m, __uint_as_float(c2 ? ml[e][k].z : ml[e][k].x));
-                        const float c = m == -INFINITY ? 0.f : m, a = exp2_fast(M[e][c2] - c);
+                        const float c = m == -INFINITY ? 0.f : m, a = weight_of(M[e][c2], c);
                         M[e][c2] = m;
                         l[e][c2] *= a; x[e][c2] *= a; x[e][2 + c2] *= a;
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            const float a1 = exp2_fast(__uint_as_float(c2 ? ml[e][k].z : ml[e][k].x) - c);
+                            const float a1 = weight_of(__uint_as_float(c2 ? ml[e][k].z : ml[e][k].x), c);
                             l[e][c2] += __uint_as_float(c2 ? ml[e][k].w : ml[e][k].y) * a1;
                             x[e][c2] += __uint_as_float(c2 ? y[e][k].y : y[e][k].x) * a1;
                             x[e][2 + c2] += __uint_as_float(c2 ? y[e][k].w : y[e][k].z) * a1;
@@ -759,7 +764,7 @@ struct KvAttendWork {
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float a = exp2_fast(M[i >> 1][i & 1] - (all[i >> 1][i & 1] == -INFINITY ? 0.f : all[i >> 1][i & 1]));
+                const float a = weight_of(M[i >> 1][i & 1], all[i >> 1][i & 1] == -INFINITY ? 0.f : all[i >> 1][i & 1]);
                 l[i >> 1][i & 1] *= a; x[i >> 1][i & 1] *= a; x[i >> 1][2 + (i & 1)] *= a;
             }
 #pragma unroll 1
@@ -877,8 +882,8 @@ static int launch_attend_nt(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     w.table = p->block_table; w.table_stride = p->table_stride; w.table_width = p->table_width; w.lens = p->seq_lens;
     w.batch = p->batch; w.n_q_heads = p->n_q_heads;
     w.group = p->n_q_heads / L.n_kv_heads; w.tiles = (w.group + KV_ROWS - 1) / KV_ROWS;
-    /* never 0: -infinity x 0, of a score that is not visible, would be NaN */
-    w.scale_log2 = fmaxf(fabsf(p->scale) * 1.4426950408889634f, 1e-30f);
+    /* neither 0 nor infinite: -infinity x 0, of a score that is not visible, and 0 x infinity, of the largest, would be NaN */
+    w.scale_log2 = fminf(fmaxf(fabsf(p->scale) * 1.4426950408889634f, FLT_TRUE_MIN), FLT_MAX);
     w.q_sign = p->scale < 0.f ? 0x80008000u : 0u;
     w.window = p->window < 0x7fffffff ? (uint32_t)p->window : 0x7fffffffu;
     w.sinks = p->sinks < 0x7fffffff ? (uint32_t)p->sinks : 0x7fffffffu;
