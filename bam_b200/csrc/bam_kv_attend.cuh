@@ -435,7 +435,8 @@ struct KvAttendWork {
     /* One chunk: S = Q K^T, p = 2^((S - m) scale log2(e)), O^T += V^T p^T.  m is a maximum of S as it is, and the difference
      * comes before the scale: the largest weight is 1 however large the scores are.  (With a scaled m it would be 2 to the
      * rounding of m, anything beyond 2^24.)  The weights go into the product as two 16-bit
-     * parts, p = hi + lo, which keeps 16 (bf16) or more bits of them: the product runs twice, on a pipe that idles.
+     * parts, kv_type::weight p = hi + lo, which keeps 16 bits of them (bf16), or 21 and what is above 2^-40 (fp16): the
+     * product runs twice, on a pipe that idles.  The sums are of the same scale, the denominator counts p itself.
      * There is one copy of this code, for whole chunks and others: code that runs once a unit runs from a cold
      * instruction cache, at a microsecond for every few kilobytes. */
     BAM_DEV void chunk(state_t& z, const uint32_t (&qa)[DMAX / 16][4], uint32_t stage, const kv_seen_t& v, uint32_t t0) const
@@ -512,9 +513,10 @@ struct KvAttendWork {
 #pragma unroll
                 for (int e = 0; e < 2; e++) p[e] = weight_of(s[i][2 * n + e], n ? c1 : c0);
                 z.l[n] += p[0] + p[1];
-                hi[n][i] = kv_type<T>::pack(p[0], p[1]);
+                const float w0 = p[0] * kv_type<T>::weight, w1 = p[1] * kv_type<T>::weight;
+                hi[n][i] = kv_type<T>::pack(w0, w1);
                 const float2 h = kv_type<T>::unpack(hi[n][i]);
-                lo[n][i] = kv_type<T>::pack(p[0] - h.x, p[1] - h.y);
+                lo[n][i] = kv_type<T>::pack(w0 - h.x, w1 - h.y);
             }
         }
 #pragma unroll
@@ -539,6 +541,8 @@ struct KvAttendWork {
         if (o32) *reinterpret_cast<uint32_t*>(p) = w;
         else { p[0] = (uint16_t)w; p[1] = (uint16_t)(w >> 16); }
     }
+    /* what the sums are multiplied with in the end */
+    BAM_DEV static float inverse(float l) { return l == 0.f ? 0.f : (1.f / kv_type<T>::weight) / l; }
     BAM_DEV float lse_of(float m, float l) const { return m == -INFINITY ? -INFINITY : m * scale_log2 * 0.69314718055994531f + logf(l); }
 
     /* the unit's result from one warp's registers */
@@ -546,7 +550,7 @@ struct KvAttendWork {
     {
         const uint32_t lane = lane_id(), h = u / tiles, r0 = (u - h * tiles) * KV_ROWS;
         float inv[NT][2];
-        to_columns(z.l[0] == 0.f ? 0.f : 1.f / z.l[0], z.l[1] == 0.f ? 0.f : 1.f / z.l[1], inv);
+        to_columns(inverse(z.l[0]), inverse(z.l[1]), inv);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -783,7 +787,7 @@ struct KvAttendWork {
                     const int e = i >> 1, c2 = i & 1;
                     if (act[e] && q0[e] + c2 < rows) {
                         const uint32_t hq = h * group + r0 + q0[e] + c2, d = gi[e] / 32 % (D / 16) * 16 + (gi[e] >> 2) % 8;
-                        const float inv = l[e][c2] == 0.f ? 0.f : 1.f / l[e][c2];
+                        const float inv = inverse(l[e][c2]);
                         uint16_t* dst = out + b * o_sb + hq * o_sh + d;
                         const uint32_t w = kv_type<T>::pack(x[e][c2] * inv, x[e][2 + c2] * inv);
                         dst[0] = (uint16_t)w;

@@ -1,9 +1,81 @@
-"""GPU tests of the key/value cache where its attention's numbers get hard."""
+"""GPU tests of the key/value cache where its attention's numbers get hard.
+
+Tolerances beyond those of test_gpu_kv: the weights of an fp16 product are kept to 2^-40 of the largest, or to 2^-16 of
+themselves where that is more, so n of them with values up to V are off by n * 2^-40 * V in all."""
 import pytest
 
 from test_gpu_kv import done, fill, make
 
 pytestmark = pytest.mark.gpu
+
+
+def led(torch, g, kv, lens, table, lead, below, spread, v):
+    """Keys whose scores against the query `8, 0, 0, ...` at scale 1 are 0 at token `lead(n)` of each sequence and between
+    -below and -below - spread nats elsewhere; they are exact in 64 bits and in 32."""
+    T = kv.block_tokens
+    k = torch.zeros_like(v)
+    x = -(below + spread * torch.rand(len(k), kv.n_kv_heads, generator=g, device="cuda")) / 8
+    k[..., 0] = x.to(kv.dtype)
+    at = [table[b].long()[lead(n) // T] * T + lead(n) % T for b, n in enumerate(lens)]
+    for i in at:
+        k[i] = 0
+    return k, at
+
+
+def close_led(torch, got, ref, lens, dtype, vmax):
+    """Scores and their differences are single products, rounded once or twice: 2^-22 of their size; a weight is kept to
+    2^-16 of itself or 2^-40 of the largest; sums as in test_gpu_kv.  The rounding to the type comes last."""
+    out, a, smax = ref
+    n = torch.tensor(lens, dtype=torch.float64, device="cuda")[:, None, None]
+    rel = 2 * smax * 2.0 ** -22 + 2.0 ** -16 + n.clamp(max=1024) * 2.0 ** -22
+    tol = a * rel + n * 2.0 ** -40 * vmax
+    tol = tol + torch.finfo(dtype).eps / 2 * (out.abs() + tol) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    err = (got.double() - out).abs()
+    assert torch.isfinite(got).all() and (err <= tol).all(), f"worst {float((err / tol).max())} x the tolerance"
+
+
+def weighted64(torch, q, k, v, table, lens, T):
+    """(out, sum of the magnitudes, largest score) at scale 1, in 64 bits."""
+    B, HQ, D = q.shape
+    H = k.shape[1]
+    out, a = torch.zeros(B, HQ, D, dtype=torch.float64, device="cuda"), torch.zeros(B, HQ, D, dtype=torch.float64, device="cuda")
+    smax = torch.zeros(B, HQ, 1, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        rows = table[b].long()[j // T] * T + j % T
+        s = torch.einsum("hgd,nhd->hgn", q[b].double().view(H, HQ // H, D), k[rows].double())
+        p = torch.softmax(s, -1)
+        out[b] = torch.einsum("hgn,nhd->hgd", p, v[rows].double()).reshape(HQ, D)
+        a[b] = torch.einsum("hgn,nhd->hgd", p, v[rows].double().abs()).reshape(HQ, D)
+        smax[b] = s.abs().amax(-1).reshape(HQ, 1)
+    return out, a, smax
+
+
+@pytest.mark.parametrize("dtype_name", ["float16", "bfloat16"])
+@pytest.mark.parametrize("dim, group, where, below, spread", [
+    (64, 4, "first", 15.5, 0.4), (128, 8, "first", 17.4, 0.0), (128, 9, "middle", 16.0, 3.0), (256, 2, "first", 11.0, 9.0),
+    (48, 3, "last", 17.0, 1.5), (96, 1, "last", 14.0, 6.0),
+])
+def test_small_weights_beside_a_large_one(cuda, bam, dtype_name, dim, group, where, below, spread):
+    """One token leads by 11 to 20 nats and has a value of zero, as the first token of a sequence often does: the output is
+    what thousands of small weights make of their values.  Few workers, so that one run holds the leader and many others."""
+    torch = cuda
+    dtype = getattr(torch, dtype_name)
+    g = torch.Generator(device="cuda").manual_seed(dim + group)
+    lens = [8000, 1500, 33]
+    kv = make(bam, torch, sum(-(-n // 16) for n in lens) + 4, 1, dim, dtype, tokens=16, max_grid=3)
+    _, v, table = fill(torch, g, kv, lens)
+    v = (v.float().abs() + 0.5).to(dtype)
+    lead = {"first": lambda n: 0, "middle": lambda n: n // 2, "last": lambda n: n - 1}[where]
+    k, at = led(torch, g, kv, lens, table, lead, below, spread, v)
+    for i in at:
+        v[i] = 0
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    q = torch.zeros(len(lens), group, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 8
+    got = kv.attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), scale=1.0)
+    close_led(torch, got, weighted64(torch, q, k, v, table, lens, 16), lens, dtype, float(v.abs().max()))
+    done(kv)
 
 
 @pytest.mark.parametrize("scale", [1.0, 0.3, -0.7])
