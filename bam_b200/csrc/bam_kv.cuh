@@ -77,13 +77,11 @@ struct kv_layout_d_t {
 template <class T> struct kv_type;
 template <> struct kv_type<__nv_bfloat16> {
     static constexpr float weight = 1.f;
-    static BAM_DEV float to_f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
     static BAM_DEV uint32_t pack(float lo, float hi) { __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&p); }
     static BAM_DEV float2 unpack(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 };
 template <> struct kv_type<__half> {
     static constexpr float weight = 32768.f;
-    static BAM_DEV float to_f(uint16_t b) { return __half2float(__ushort_as_half(b)); }
     static BAM_DEV uint32_t pack(float lo, float hi) { __half2 p = __floats2half2_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&p); }
     static BAM_DEV float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 };
