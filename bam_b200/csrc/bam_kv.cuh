@@ -73,15 +73,21 @@ struct kv_layout_d_t {
 
 /* weight: what the softmax weights, 1 at most, are multiplied with for the product with the values.  fp16 has no number
  * between 0 and 2^-24, but thousands of weights of that size beside one of 1 are a part of the output that it can tell from
- * none; 2^15 is the largest power of two below its maximum.  bf16 has the range of 32 bits. */
+ * none; 2^15 is the largest power of two below its maximum.  bf16 has the range of 32 bits.
+ * positive: both elements of a weight (none is negative), none of them 0 for a weight that is not; in bf16 none is.
+ * finite: both elements, an infinite one as the largest number of its sign. */
 template <class T> struct kv_type;
 template <> struct kv_type<__nv_bfloat16> {
     static constexpr float weight = 1.f;
+    static BAM_DEV uint32_t positive(uint32_t u) { return u; }
+    static BAM_DEV uint32_t finite(uint32_t u) { uint32_t r; asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x7f7f7f7fu)); return r; }
     static BAM_DEV uint32_t pack(float lo, float hi) { __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&p); }
     static BAM_DEV float2 unpack(uint32_t u) { return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 };
 template <> struct kv_type<__half> {
     static constexpr float weight = 32768.f;
+    static BAM_DEV uint32_t positive(uint32_t u) { uint32_t r; asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x00010001u)); return r; }
+    static BAM_DEV uint32_t finite(uint32_t u) { uint32_t r; asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x7bff7bffu)); return r; }
     static BAM_DEV uint32_t pack(float lo, float hi) { __half2 p = __floats2half2_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&p); }
     static BAM_DEV float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 };

@@ -437,6 +437,9 @@ struct KvAttendWork {
      * rounding of m, anything beyond 2^24.)  The weights go into the product as two 16-bit
      * parts, kv_type::weight p = hi + lo, which keeps 16 bits of them (bf16), or 21 and what is above 2^-40 (fp16): the
      * product runs twice, on a pipe that idles.  The sums are of the same scale, the denominator counts p itself.
+     * An infinite value makes its sum infinite, if its weight is any number but 0 in 32 bits: infinity x 0, of a part that
+     * is 0, and infinities of different sign, of parts of different sign, would make it NaN.  So hi is never 0 (lo takes what
+     * is too much back) and lo is multiplied with values cut to the finite range.
      * There is one copy of this code, for whole chunks and others: code that runs once a unit runs from a cold
      * instruction cache, at a microsecond for every few kilobytes. */
     BAM_DEV void chunk(state_t& z, const uint32_t (&qa)[DMAX / 16][4], uint32_t stage, const kv_seen_t& v, uint32_t t0) const
@@ -514,7 +517,7 @@ struct KvAttendWork {
                 for (int e = 0; e < 2; e++) p[e] = weight_of(s[i][2 * n + e], n ? c1 : c0);
                 z.l[n] += p[0] + p[1];
                 const float w0 = p[0] * kv_type<T>::weight, w1 = p[1] * kv_type<T>::weight;
-                hi[n][i] = kv_type<T>::pack(w0, w1);
+                hi[n][i] = kv_type<T>::positive(kv_type<T>::pack(w0, w1));
                 const float2 h = kv_type<T>::unpack(hi[n][i]);
                 lo[n][i] = kv_type<T>::pack(w0 - h.x, w1 - h.y);
             }
@@ -528,6 +531,8 @@ struct KvAttendWork {
                     ldm_x4_t(r, at(v_row, v_c, mt * 2) + kt * 16 * rb);
 #pragma unroll
                     for (int n = 0; n < NT; n++) mma_16816(z.o[n][mt], r, hi[n][2 * kt], hi[n][2 * kt + 1], T());
+#pragma unroll
+                    for (int k = 0; k < 4; k++) r[k] = kv_type<T>::finite(r[k]);
 #pragma unroll
                     for (int n = 0; n < NT; n++) mma_16816(z.o[n][mt], r, lo[n][2 * kt], lo[n][2 * kt + 1], T());
                 }

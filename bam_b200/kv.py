@@ -217,7 +217,9 @@ class KvCache:
         window > 0: only the last `window` tokens and the first `sinks` are visible; blocks without a visible token are
         not touched, their table entries may be anything.  scale defaults to head_dim ** -0.5.  Returns out, or
         (out, lse) with the logarithm of the softmax's denominator [batch, heads]; a sequence with nothing visible gets
-        zeros and -inf.  The new token's own key and value have to be appended first.  `out` may be q itself."""
+        zeros and -inf.  A score of -infinity hides its token, +infinity or NaN make the head's row NaN; an infinite value
+        makes its element infinite (a weight below 2^-126 of the largest is 0, and 0 x infinity NaN).  The new token's own
+        key and value have to be appended first.  `out` may be q itself."""
         import torch
         if stream is not None:
             with self._on_stream(stream):

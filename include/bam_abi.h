@@ -412,7 +412,8 @@ int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t 
  * over the tokens j < seq_lens[b] (int32) that are visible: all of them, or with window > 0 the last `window` and the
  * first `sinks`.  Query head h reads key/value head h / (n_q_heads / n_kv_heads).  Token j of sequence b lies in block
  * block_table[b * table_stride + j / block_tokens] (int32); entries of blocks without a visible token are not read.
- * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL).  out may be q. */
+ * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL).  An infinite value of a visible
+ * token makes its element of out infinite (NaN with one of the other sign, or if p_j is below 2^-126).  out may be q. */
 typedef struct {
     const void* q;
     void* out;

@@ -4,7 +4,7 @@ Tolerances beyond those of test_gpu_kv: the weights of an fp16 product are kept 
 themselves where that is more, so n of them with values up to V are off by n * 2^-40 * V in all."""
 import pytest
 
-from test_gpu_kv import done, fill, make
+from test_gpu_kv import done, fill, make, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -75,6 +75,45 @@ def test_small_weights_beside_a_large_one(cuda, bam, dtype_name, dim, group, whe
     q[..., 0] = 8
     got = kv.attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), scale=1.0)
     close_led(torch, got, weighted64(torch, q, k, v, table, lens, 16), lens, dtype, float(v.abs().max()))
+    done(kv)
+
+
+@pytest.mark.parametrize("dtype_name, below", [("bfloat16", 0.0), ("bfloat16", 3.0), ("bfloat16", 60.0), ("bfloat16", 80.0),
+                                               ("float16", 0.0), ("float16", 5.0), ("float16", 16.0), ("float16", 40.0), ("float16", 80.0)])
+@pytest.mark.parametrize("dim, group", [(64, 2), (128, 11), (256, 3), (48, 1)])
+def test_values_that_are_infinite_in_visible_rows(cuda, bam, dtype_name, below, dim, group):
+    """An infinite value of a visible token makes its element of the output infinite, whether the token's weight is one or
+    e^-80; two of different sign, or a NaN, make it NaN; the other elements, heads and sequences do not notice."""
+    torch = cuda
+    dtype = getattr(torch, dtype_name)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    lens = [300, 90, 45, 200]
+    kv = make(bam, torch, sum(-(-n // 16) for n in lens) + 4, 2, dim, dtype, tokens=16)
+    _, v, table = fill(torch, g, kv, lens)
+    k, at = led(torch, g, kv, lens, table, lambda n: n // 3, below, 0.0 if below else 4.0, v)
+    inf, nan = float("inf"), float("nan")
+    row = lambda b, j: table[b].long()[j // 16] * 16 + j % 16           # noqa: E731
+    for j, d, x in ((5, 0, inf), (299, 1, -inf), (100, 2, inf), (100, 3, -inf), (7, 4, inf), (200, 4, -inf), (8, 5, inf), (250, 5, inf),
+                    (299, dim - 1, nan)):                               # token 100 is the leader, of weight one
+        v[row(0, j), 0, d] = x
+    for j in range(90):
+        v[row(1, j), 1, dim - 2] = -inf
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    q = torch.zeros(len(lens), 2 * group, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 8
+    got, lse = kv.attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), scale=1.0, return_lse=True)
+    want = torch.zeros(len(lens), 2 * group, dim, device="cuda")
+    want[0, :group, 0] = want[0, :group, 2] = want[0, :group, 5] = inf
+    want[0, :group, 1] = want[0, :group, 3] = -inf
+    want[0, :group, 4] = want[0, :group, dim - 1] = nan
+    want[1, group:, dim - 2] = -inf
+    odd = want != 0
+    assert torch.equal(got[odd].float().nan_to_num(123.0), want[odd].nan_to_num(123.0))
+    v = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    out, a, smax = weighted64(torch, q, k, v, table, lens, 16)
+    got = torch.where(odd, torch.zeros_like(got), got)
+    close_led(torch, got, (out.masked_fill(odd, 0), a.masked_fill(odd, 0), smax), lens, dtype, float(v.abs().max()))
+    assert torch.isfinite(lse).all()
     done(kv)
 
 
