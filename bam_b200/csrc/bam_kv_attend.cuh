@@ -548,7 +548,8 @@ struct KvAttendWork {
     }
     /* what the sums are multiplied with in the end */
     BAM_DEV static float inverse(float l) { return l == 0.f ? 0.f : (1.f / kv_type<T>::weight) / l; }
-    BAM_DEV float lse_of(float m, float l) const { return m == -INFINITY ? -INFINITY : m * scale_log2 * 0.69314718055994531f + logf(l); }
+    /* nothing visible: -infinity twice over; scores that are all NaN leave m at -infinity, and l says NaN */
+    BAM_DEV float lse_of(float m, float l) const { return m * scale_log2 * 0.69314718055994531f + logf(l); }
 
     /* the unit's result from one warp's registers */
     BAM_DEV void write_out(const state_t& z, uint32_t b, uint32_t u) const

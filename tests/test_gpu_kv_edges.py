@@ -117,6 +117,21 @@ def test_values_that_are_infinite_in_visible_rows(cuda, bam, dtype_name, below, 
     done(kv)
 
 
+@pytest.mark.parametrize("lens", [[1], [700, 1, 20]])
+def test_rows_whose_every_score_is_nan(cuda, bam, lens):
+    """The maximum of no number at all must not turn into an empty sequence's: lse is NaN like the output."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(21)
+    kv = make(bam, torch, sum(-(-n // 16) for n in lens) + 4, 1, 64, torch.bfloat16, page=4096)
+    k, v, table = fill(torch, g, kv, lens)
+    k.fill_(float("nan"))
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    q = rand(torch, g, len(lens), 3, 64, dtype=torch.bfloat16)
+    out, lse = kv.attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), return_lse=True)
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    done(kv)
+
+
 @pytest.mark.parametrize("scale", [1.0, 0.3, -0.7])
 @pytest.mark.parametrize("top", [2.0 ** 27, 2.0 ** 33, 2.0 ** 50, -2.0 ** 40, 2.0 ** 100])
 def test_scores_far_beyond_the_exponential(cuda, bam, scale, top):
