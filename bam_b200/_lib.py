@@ -107,6 +107,7 @@ SIGNATURES = {
     "bam_pagerank_run": (ci, [vp, vp, u64, u64, u64, u64, u32, vp, C.POINTER(u32), C.POINTER(u64)]),
     "bam_kv_scratch_bytes": (u64, [vp, C.POINTER(KvLayout)]),
     "bam_kv_scratch_init": (ci, [vp, vp, u64, vp]),
+    "bam_kv_stream_id": (u64, [vp]),
     "bam_launch_kv_append": (ci, [vp, C.POINTER(KvLayout), C.POINTER(KvAppend), vp, u64, vp]),
     "bam_launch_kv_gather": (ci, [vp, C.POINTER(KvLayout), u64, vp, vp, vp, C.POINTER(i64), C.POINTER(i64), vp, u64, vp]),
     "bam_launch_kv_attend": (ci, [vp, C.POINTER(KvLayout), C.POINTER(KvAttend), vp, u64, vp]),

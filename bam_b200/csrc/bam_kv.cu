@@ -482,6 +482,14 @@ extern "C" int bam_kv_scratch_init(bam_array_t a, void* scratch_dev, uint64_t sc
     return BAM_OK;
 }
 
+extern "C" uint64_t bam_kv_stream_id(void* stream)
+{
+    unsigned long long id = 0;
+    if (cudaStreamGetId((cudaStream_t)stream, &id) == cudaSuccess) return id;
+    (void)cudaGetLastError();
+    return ~0ull;
+}
+
 static int check_scratch(bam_array_t a, const bam_kv_layout_t* layout, void* scratch, uint64_t scratch_bytes)
 {
     if (!scratch || ((uintptr_t)scratch & 127)) return BAM_EINVAL;

@@ -14,14 +14,9 @@ from .host import REPLICATE, Array
 ROPE_STYLES = {"half": 0, "pairs": 1}
 
 _NO_STRIDE = (0, 0)
-_scratch = {}       # (device, stream) -> the scratch memory of the launches on that stream
-
-
-def _raw_stream(index):
-    """The handle of torch's current stream (by the short way where this torch has it: a call takes 15 us in all)."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+_PER_THREAD = 2     # cudaStreamPerThread
+_NO_STREAM = (1 << 64) - 1
+_scratch = {}       # (device, stream) -> the stream's number, the scratch memory of the launches on that stream
 
 
 class KvCache:
@@ -33,7 +28,9 @@ class KvCache:
 
     The calls run on the current stream of the cache's device or on `stream` (a torch stream or a raw handle), in whose
     memory pool their results are; the order between streams, and that tensors live long enough, is the caller's affair as
-    for any work on another stream.  They may be captured into CUDA graphs.  Results carry no gradient."""
+    for any work on another stream.  (The per-thread default stream is refused: its handle is the same number in every
+    thread, and torch's memory pools take it for one stream.)  They may be captured into CUDA graphs.  Results carry no
+    gradient."""
 
     def __init__(self, cache, n_blocks, n_kv_heads, head_dim, dtype=None, block_tokens=None, n_layers=1, store_byte_offset=0,
                  dist=REPLICATE):
@@ -60,6 +57,10 @@ class KvCache:
         self._layouts = [C.byref(KvLayout(0 if dtype == torch.bfloat16 else 1, head_dim, n_kv_heads, block_tokens, n_blocks,
                                           i * n_blocks * n_kv_heads)) for i in range(n_layers)]
         self._scratch_bytes = self.lib.bam_kv_scratch_bytes(self.array.h, self._layouts[0])
+        # what every call asks torch, by the short ways where this torch has them: a call takes 13 us in all
+        self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        self._capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     def close(self):
         self.array.close()
@@ -104,28 +105,49 @@ class KvCache:
         """`stream` (a torch stream or a raw handle) as the context the call takes its memory and runs in."""
         import torch
         if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(stream), device=self.device)
+            stream = (stream.value or 0) if isinstance(stream, C.c_void_p) else int(stream)
+            if stream == _PER_THREAD:
+                raise ValueError("the per-thread default stream is not supported")
+            stream = torch.cuda.ExternalStream(stream, device=self.device)
         if stream.device != self.device:
             raise ValueError(f"the stream is on {stream.device}, the cache on {self.device}")
         return torch.cuda.stream(stream)
 
-    def _call(self, launch, layer, *args):
-        """A launch on the current stream of the cache's device.  Scratch memory belongs to the stream, whose launches run
-        one after the other (and share it between all caches of the device); a captured launch has its own, which belongs
-        to its graph."""
+    def _new_scratch(self, stream):
         import torch
+        scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=self.device)
+        check(self.lib.bam_kv_scratch_init(self.array.h, scratch.data_ptr(), self._scratch_bytes, stream), "bam_kv_scratch_init")
+        return scratch
+
+    def _scratch_of(self, stream):
+        """The scratch memory of a stream, whose launches run one after the other (and share it between all caches of the
+        device).  A handle may be given out again when its stream is gone, possibly while that one's last launch still runs;
+        the number of a stream is its own."""
+        if stream == _PER_THREAD:
+            raise ValueError("the per-thread default stream is not supported")
+        number = self.lib.bam_kv_stream_id(stream)
+        had, scratch = _scratch.get((self.device.index, stream), (number, None))
+        if number == _NO_STREAM:
+            raise RuntimeError(f"{stream:#x} is no stream")
+        if had != number:
+            import torch
+            torch.cuda.synchronize(self.device)
+            scratch = None
+        if scratch is None or scratch.numel() < self._scratch_bytes:
+            scratch = self._new_scratch(stream)
+            _scratch[self.device.index, stream] = number, scratch
+        return scratch
+
+    def _call(self, launch, layer, *args):
+        """A launch on the current stream of the cache's device, with scratch memory that no launch uses at the same time: that
+        of the stream, or, for a captured launch, its own, which belongs to its graph."""
         index = self.device.index
-        if torch.cuda.current_device() != index:
+        if self._current_device() != index:
+            import torch
             with torch.cuda.device(index):
                 return self._call(launch, layer, *args)
-        stream = _raw_stream(index)
-        capturing = torch.cuda.is_current_stream_capturing()
-        scratch = None if capturing else _scratch.get((index, stream))
-        if scratch is None or scratch.numel() < self._scratch_bytes:
-            scratch = torch.empty(self._scratch_bytes, dtype=torch.uint8, device=self.device)
-            check(self.lib.bam_kv_scratch_init(self.array.h, scratch.data_ptr(), self._scratch_bytes, stream), "bam_kv_scratch_init")
-            if not capturing:
-                _scratch[index, stream] = scratch
+        stream = self._raw_stream(index)
+        scratch = self._new_scratch(stream) if self._capturing() else self._scratch_of(stream)
         check(launch(self.array.h, layer, *args, scratch.data_ptr(), self._scratch_bytes, stream), launch.__name__)
 
     # ---- operators ----------------------------------------------------------------------------------------

@@ -365,7 +365,8 @@ int bam_ctrl_write_store_from_device(bam_ctrl_t c, uint64_t byte_offset, const v
  * contiguous.  Every launch is asynchronous on `stream`, may be captured into a CUDA graph, and leaves the calling
  * thread's device as it was.  scratch_dev: bam_kv_scratch_bytes bytes of device memory, 128-byte aligned, set up once
  * by bam_kv_scratch_init.  Every launch leaves it ready for the next, also one that fails; launches that may run at the
- * same time need one each: one for every stream, one for every captured graph.  An index outside its range (a slot,
+ * same time need one each: one for every stream (the handle cudaStreamPerThread is another stream in every thread), one for
+ * every captured graph.  An index outside its range (a slot,
  * position, block or length) is not followed: the status block says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has
  * finished, the rows that it concerns are undefined.  While the status block says anything, launches do nothing. */
 #define BAM_KV_BF16 0u
@@ -379,6 +380,9 @@ typedef struct {
 } bam_kv_layout_t;
 uint64_t bam_kv_scratch_bytes(bam_array_t a, const bam_kv_layout_t* layout);
 int bam_kv_scratch_init(bam_array_t a, void* scratch_dev, uint64_t scratch_bytes, void* stream);
+/* The number of a stream of the current device, which no other stream of the process ever has (a handle may be given out
+ * again when its stream is gone); ~0 if it has none. */
+uint64_t bam_kv_stream_id(void* stream);
 
 /* Append: row t of k and v goes to slots[t] (int64; negative: the row is padding and nothing is written; slots are
  * distinct otherwise: of two rows for one slot neither is sure to be kept whole).  On the way each head of k, and of q

@@ -4,7 +4,7 @@ Tolerances beyond those of test_gpu_kv: the weights of an fp16 product are kept 
 themselves where that is more, so n of them with values up to V are off by n * 2^-40 * V in all."""
 import pytest
 
-from test_gpu_kv import done, fill, make, rand
+from test_gpu_kv import attend64, check_attend, done, fill, make, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -163,4 +163,37 @@ def test_scores_far_beyond_the_exponential(cuda, bam, scale, top):
         s = float(k[two[0], 0, 0].double()) * float(q[b, 0, 0].double()) * scale
         # products with the scale and the logarithm's base: three roundings and the rounded constants
         assert ((lse[b].double() - s).abs() <= 6 * 2.0 ** -24 * abs(s) + 1).all()
+    done(kv)
+
+
+def test_streams_that_come_and_go(cuda, bam):
+    """Streams that are destroyed behind a call, whose handles come back: each has a number of its own, and no two launches
+    that run at once have the same scratch memory."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(26)
+    lens = [900, 20, 400]
+    kv = make(bam, torch, 90, 2, 64, torch.bfloat16, page=4096)
+    k, v, table = fill(torch, g, kv, lens)
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    q = rand(torch, g, 3, 8, 64, dtype=torch.bfloat16, scale=2.0)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ref = attend64(torch, q, k, v, table, lens, kv.block_tokens, 0.125)
+    torch.cuda.synchronize()
+    rt, at = torch.cuda.cudart(), torch.zeros(1, dtype=torch.int64)
+    outs, numbers = [], set()
+    for _ in range(40):
+        assert int(rt.cudaStreamCreate(at.data_ptr())) == 0
+        handle = int(at)
+        numbers.add(kv.lib.bam_kv_stream_id(handle))
+        outs.append(kv.attend(q, table, ls, stream=handle))
+        outs.append(kv.attend(q, table, ls))                     # at the same time on the current stream
+        assert int(rt.cudaStreamDestroy(handle)) == 0
+    torch.cuda.synchronize()
+    assert len(numbers) == 40 and (1 << 64) - 1 not in numbers
+    assert kv.lib.bam_kv_stream_id(0) not in numbers
+    for o in outs:
+        check_attend(torch, o, None, ref, torch.bfloat16)
+    with pytest.raises(ValueError, match="per-thread"):
+        kv.attend(q, table, ls, stream=2)
+    assert kv.cache.ctrl.status() == (0, "none", 0)
     done(kv)
