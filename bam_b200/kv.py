@@ -6,6 +6,8 @@ PageCache.flush).  The calls are asynchronous like every other launch: what goes
 out, an index outside its range -- is reported by Controller.status() / check_status().
 """
 import ctypes as C
+import threading
+import weakref
 
 from . import _lib
 from ._lib import KvAppend, KvAttend, KvLayout, check
@@ -17,6 +19,7 @@ _NO_STRIDE = (0, 0)
 _PER_THREAD = 2     # cudaStreamPerThread
 _NO_STREAM = (1 << 64) - 1
 _scratch = {}       # (device, stream) -> the stream's number, the scratch memory of the launches on that stream
+_open, _open_lock = weakref.WeakSet(), threading.RLock()      # (a collection in the midst of it may close another cache)
 
 
 class KvCache:
@@ -56,6 +59,8 @@ class KvCache:
         self.array = Array(cache, n_layers * n_blocks * n_kv_heads * (cache.page_size // 8), 8, store_byte_offset, dist)
         self._layouts = [C.byref(KvLayout(0 if dtype == torch.bfloat16 else 1, head_dim, n_kv_heads, block_tokens, n_blocks,
                                           i * n_blocks * n_kv_heads)) for i in range(n_layers)]
+        with _open_lock:
+            _open.add(self)
         self._scratch_bytes = self.lib.bam_kv_scratch_bytes(self.array.h, self._layouts[0])
         # what every call asks torch, by the short ways where this torch has them: a call takes 13 us in all
         self._current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -63,7 +68,19 @@ class KvCache:
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     def close(self):
+        """Waits for the device.  The streams' scratch memory (15 MB each with heads of 128) goes with its last cache."""
         self.array.close()
+        with _open_lock:
+            _open.discard(self)
+            if not any(kv.device == self.device for kv in _open):
+                for key in [key for key in _scratch if key[0] == self.device.index]:
+                    _scratch.pop(key, None)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
     # ---- arguments ----------------------------------------------------------------------------------------
 

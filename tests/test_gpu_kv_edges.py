@@ -197,3 +197,40 @@ def test_streams_that_come_and_go(cuda, bam):
         kv.attend(q, table, ls, stream=2)
     assert kv.cache.ctrl.status() == (0, "none", 0)
     done(kv)
+
+
+def test_scratch_is_given_back(cuda, bam):
+    """The streams' scratch memory goes with the last cache of the device; a captured graph keeps its own."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(27)
+    lens = [200, 3]
+
+    def cache():
+        kv = make(bam, torch, 24, 2, 64, torch.bfloat16, page=4096)
+        k, v, table = fill(torch, g, kv, lens)
+        kv.append(k, v, torch.arange(len(k), device="cuda"))
+        return kv, k, v, table
+    q = rand(torch, g, 2, 4, 64, dtype=torch.bfloat16)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(2):
+        one, two = cache(), cache()
+        size = one[0]._scratch_bytes
+        held = torch.cuda.memory_allocated()
+        kept = one[0].attend(q, one[3], ls, stream=side)
+        assert torch.cuda.memory_allocated() - held >= size      # the side stream's
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = one[0].attend(q, one[3], ls)
+        graph.replay()
+        done(two[0])
+        ref = attend64(torch, q, one[1], one[2], one[3], lens, one[0].block_tokens, 0.125)
+        for o in (kept, out, one[0].attend(q, one[3], ls)):
+            check_attend(torch, o, None, ref, torch.bfloat16)
+        torch.cuda.synchronize()
+        del graph, out, o, kept, ref
+        done(one[0])
+        del one, two
+        assert torch.cuda.memory_allocated() - before < size

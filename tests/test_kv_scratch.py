@@ -32,11 +32,13 @@ def caches(bam, monkeypatch):
     from bam_b200 import kv as module
     lib, waits = _Lib(), []
     monkeypatch.setattr(module, "_scratch", {})
+    monkeypatch.setattr(module, "_open", type(module._open)())
     monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: waits.append(device))
 
     def make(size=256):
         k = bam.KvCache.__new__(bam.KvCache)
         k.lib, k.array, k.device, k._scratch_bytes = lib, _Array(), torch.device("cpu"), size
+        module._open.add(k)
         return k
     make.lib, make.waits, make.module = lib, waits, module
     return make
@@ -86,3 +88,24 @@ def test_the_per_thread_stream_is_refused_as_the_current_one(caches):
     caches.lib.ids = {2: 5}
     with pytest.raises(ValueError, match="per-thread"):
         caches()._scratch_of(2)
+
+
+def test_scratch_goes_with_the_last_cache_of_its_device(caches):
+    import torch
+    one, two, lib = caches(), caches(), caches.lib
+    lib.ids = {0x500: 7}
+    far = torch.zeros(8)
+    caches.module._scratch[3, 0x500] = 9, far                   # another device's
+    one._scratch_of(0x500)
+    one.close()
+    assert len(caches.module._scratch) == 2                      # `two` may want it
+    one.close()
+    assert one.array.closed == 2 and len(caches.module._scratch) == 2
+    two.close()
+    assert list(caches.module._scratch) == [(3, 0x500)]
+    # a cache that is made later starts anew, and one that nobody closes goes when it is collected
+    three = caches()
+    assert three._scratch_of(0x500).numel() == 256 and len(lib.made) == 2
+    array = three.array
+    del three
+    assert array.closed == 1 and list(caches.module._scratch) == [(3, 0x500)]
