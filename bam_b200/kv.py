@@ -110,6 +110,13 @@ class KvCache:
             raise ValueError(f"the elements of a head of {name} must be contiguous")
         return stride[:2]
 
+    def _rows(self, name, t, n, heads):
+        """The same of a tensor that is written."""
+        stride = self._heads(name, t, n, heads)
+        if (n > 1 and stride[0] < self.head_dim) or (heads > 1 and stride[1] < self.head_dim):
+            raise ValueError(f"the rows of {name} lie on one another")
+        return stride
+
     def _flat(self, name, t, dtype, n):
         """The address of n contiguous values."""
         if not (t.dtype is dtype and t.shape == (n,) and t.is_contiguous() and t.device == self.device):
@@ -220,7 +227,7 @@ class KvCache:
                 q_out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
                 out_stride = heads * self.head_dim, self.head_dim
             else:
-                out_stride = self._heads("q_out", q_out, n, heads)
+                out_stride = self._rows("q_out", q_out, n, heads)
             q_at, out_at = q.data_ptr(), q_out.data_ptr()
         if n:
             a = KvAppend(q_at, k.data_ptr(), v.data_ptr(), out_at, q_stride, k_stride, v_stride, out_stride, n, at, *turn[:5],
@@ -243,8 +250,8 @@ class KvCache:
             ks = vs = (C.c_int64 * 2)(self.n_kv_heads * self.head_dim, self.head_dim)
         else:
             k, v = out
-            ks = (C.c_int64 * 2)(*self._heads("out[0]", k, n, self.n_kv_heads))
-            vs = (C.c_int64 * 2)(*self._heads("out[1]", v, n, self.n_kv_heads))
+            ks = (C.c_int64 * 2)(*self._rows("out[0]", k, n, self.n_kv_heads))
+            vs = (C.c_int64 * 2)(*self._rows("out[1]", v, n, self.n_kv_heads))
         if n:
             self._call(self.lib.bam_launch_kv_gather, layout, n, at, k.data_ptr(), v.data_ptr(), ks, vs)
         return k, v
@@ -279,7 +286,7 @@ class KvCache:
             out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
             out_stride = heads * self.head_dim, self.head_dim
         else:
-            out_stride = self._heads("out", out, n, heads)
+            out_stride = self._rows("out", out, n, heads)
         lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
         if n:
             a = KvAttend(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, q_stride, out_stride, block_table.data_ptr(),
