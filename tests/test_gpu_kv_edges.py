@@ -166,6 +166,67 @@ def test_scores_far_beyond_the_exponential(cuda, bam, scale, top):
     done(kv)
 
 
+@pytest.mark.parametrize("rising", [6.0, -6.0, 200.0])
+def test_a_sequence_shared_by_more_workers_than_join_at_once(cuda, bam, rising):
+    """40000 tokens of one key/value head are more than 128 workers' parts: the join takes them in rounds, and the maximum
+    moves between the rounds."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(23)
+    lens, dim = [40000, 37001], 64
+    kv = make(bam, torch, sum(-(-n // 256) for n in lens) + 4, 1, dim, torch.bfloat16, page=65536)
+    k, v, table = fill(torch, g, kv, lens)
+    T = kv.block_tokens
+    q = rand(torch, g, 2, 3, dim, dtype=torch.bfloat16)
+    q[..., 0] = 8
+    for b, n in enumerate(lens):
+        j = torch.arange(n, device="cuda")
+        k[table[b].long()[j // T] * T + j % T, 0, 0] = (rising * j / n / (8 * dim ** -0.5)).bfloat16()
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    out, lse = kv.attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), return_lse=True)
+    check_attend(torch, out, lse, attend64(torch, q, k, v, table, lens, T, dim ** -0.5), torch.bfloat16)
+    done(kv)
+
+
+def test_more_sequences_than_a_scan_of_the_lengths(cuda, bam):
+    """5000 sequences, many of them empty: each thread that lays out the list counts more than 32."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(24)
+    B, dim = 5000, 64
+    kv = make(bam, torch, 64, 2, dim, torch.bfloat16, page=4096)
+    T = kv.block_tokens
+    k, v = rand(torch, g, 64 * T, 2, dim, dtype=torch.bfloat16), rand(torch, g, 64 * T, 2, dim, dtype=torch.bfloat16)
+    kv.append(k, v, torch.arange(64 * T, device="cuda"))
+    table = torch.randint(0, 64, (B, 3), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.randint(0, 3 * T + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lens[torch.rand(B, generator=g, device="cuda") < 0.4] = 0
+    lens[1000:1100] = 0
+    q = rand(torch, g, B, 4, dim, dtype=torch.bfloat16, scale=2.0)
+    out, lse = kv.attend(q, table, lens, return_lse=True)
+    check_attend(torch, out, lse, attend64(torch, q, k, v, table, lens.tolist(), T, dim ** -0.5), torch.bfloat16)
+    done(kv)
+
+
+@pytest.mark.parametrize("dim, page, slots, grid", [(128, 16384, 60, 4), (256, 16384, 700, 0), (48, 4096, 50, 3)])
+def test_fp16_attention_from_the_store(cuda, bam, dim, page, slots, grid):
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(25)
+    lens = [1300, 3, 0, 700]
+    T = page // (4 * dim) // 16 * 16
+    kv = make(bam, torch, sum(-(-n // T) for n in lens) + 3, 2, dim, torch.float16, page=page, slots=slots, max_grid=grid)
+    k, v, table = fill(torch, g, kv, lens)
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    kv.cache.flush()
+    kv.cache.invalidate()
+    q = rand(torch, g, len(lens), 6, dim, dtype=torch.float16, scale=2.0)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for window, sinks in ((0, 0), (200, 5)):
+        out, lse = kv.attend(q, table, ls, window=window, sinks=sinks, return_lse=True)
+        check_attend(torch, out, lse, attend64(torch, q, k, v, table, lens, T, dim ** -0.5, window, sinks), torch.float16)
+    assert kv.cache.ctrl.status() == (0, "none", 0)
+    assert kv.cache.stats()["read_ios"] > 0
+    done(kv)
+
+
 def test_streams_that_come_and_go(cuda, bam):
     """Streams that are destroyed behind a call, whose handles come back: each has a number of its own, and no two launches
     that run at once have the same scratch memory."""
