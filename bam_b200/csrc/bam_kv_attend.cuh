@@ -251,6 +251,7 @@ struct KvAttendWork {
         const uint32_t end = works ? sh.chunks[w] : 0;
         kv_place_t at = sh.from[w];                       /* where chunk `next` of the worker is */
         uint32_t next = 0, ask = most;                    /* chunks asked for at a time: fewer in a cache that is too full for all */
+        bool alone = false;                               /* one worker's next chunk and nothing else: no chunk could be had whole */
         spin_t sp;
         for (;;) {
             const uint32_t n = next + c, round = n / ahead, place = n - round * ahead;
@@ -263,6 +264,7 @@ struct KvAttendWork {
             if (!__any_sync(full_mask, mine)) return;     /* all runs are pinned */
             const uint32_t gap = ~__ballot_sync(full_mask, mine) & mask;                 /* (the places come free in order) */
             if (gap && lane > (uint32_t)__ffs(gap) - 1u) mine = false;
+            if (alone && ((__ballot_sync(full_mask, mine) & ((1u << lane) - 1u) & ~mask) || c > 0)) mine = false;
             uint32_t b = at.b, rows = 0, slot = BAM_SLOT_NONE;
             uint64_t pos = at.pos + c, page = 0, offset = 0;
             bool want = false;
@@ -314,7 +316,8 @@ struct KvAttendWork {
             const uint64_t lpos = __shfl_sync(full_mask, pos, last);
             if (ready) { next += ready; at.b = lb; at.pos = lpos + 1; }
             ask = miss ? (ask + 1) / 2 : (ask * 2 < most ? ask * 2 : most);
-            if (!__any_sync(full_mask, ready)) {
+            alone = !__any_sync(full_mask, ready);
+            if (alone) {
                 if (__any_sync(full_mask, sp.expired(L.r.cache.status, BAM_AT_FIND_SLOT, page))) { sh.abort = 1; return; }
             } else sp.reset();
         }
@@ -904,6 +907,7 @@ static int launch_attend_nt(bam_array* a, const kv_layout_d_t& L, const bam_kv_a
     w.arrived = (uint32_t*)(base + sizeof(kv_launch_words_t));
     w.parts = (float*)(base + kv_parts_at(most * KV_WORKERS));
     w.piece = L.block_tokens % CS == 0 ? CS : 16;
+    if (a->pc->d.n_slots < CS / w.piece) return BAM_EINVAL;                               /* a chunk's pages are pinned together */
     /* no more blocks than the longest sequences could keep busy */
     uint64_t chunks = ((uint64_t)p->table_width * L.block_tokens + CS - 1) / CS;
     if (chunks > 0x80000000u / CS) chunks = 0x80000000u / CS;                             /* lengths are 32-bit numbers */

@@ -417,7 +417,8 @@ int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t 
  * first `sinks`.  Query head h reads key/value head h / (n_q_heads / n_kv_heads).  Token j of sequence b lies in block
  * block_table[b * table_stride + j / block_tokens] (int32); entries of blocks without a visible token are not read.
  * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL).  An infinite value of a visible
- * token makes its element of out infinite (NaN with one of the other sign, or if p_j is below 2^-126).  out may be q. */
+ * token makes its element of out infinite (NaN with one of the other sign, or if p_j is below 2^-126).  out may be q.  A cache
+ * of a single slot is refused where block_tokens is no multiple of 32: two blocks are read together there. */
 typedef struct {
     const void* q;
     void* out;

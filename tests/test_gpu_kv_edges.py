@@ -295,3 +295,46 @@ def test_scratch_is_given_back(cuda, bam):
         done(one[0])
         del one, two
         assert torch.cuda.memory_allocated() - before < size
+
+
+@pytest.mark.parametrize("slots, page, grid", [(1, 4096, 3), (1, 8192, 3), (2, 4096, 3), (3, 4096, 3), (5, 8192, 3), (3, 4096, 5), (6, 4096, 0)])
+def test_caches_of_a_few_slots(cuda, bam, slots, page, grid):
+    """Blocks of 16 tokens are read in pairs, which takes two slots; a single one is refused and not waited for."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(28)
+    lens = [100, 1, 33]
+    kv = make(bam, torch, 16, 2, 64, torch.bfloat16, page=page, slots=slots, max_grid=grid)
+    kv.cache.ctrl.configure(spin_timeout_ns=2_000_000_000)
+    k, v, table = fill(torch, g, kv, lens)
+    kv.append(k, v, torch.arange(len(k), device="cuda"))
+    bk, bv = kv.gather(torch.arange(len(k), device="cuda"))
+    assert torch.equal(bk, k) and torch.equal(bv, v)
+    q = rand(torch, g, len(lens), 4, 64, dtype=torch.bfloat16)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    if slots == 1 and kv.block_tokens == 16:
+        with pytest.raises(RuntimeError, match="bam_launch_kv_attend"):
+            kv.attend(q, table, ls)
+    else:
+        out, lse = kv.attend(q, table, ls, return_lse=True)
+        assert kv.cache.ctrl.status() == (0, "none", 0)
+        check_attend(torch, out, lse, attend64(torch, q, k, v, table, lens, kv.block_tokens, 0.125), torch.bfloat16)
+    done(kv)
+
+
+@pytest.mark.parametrize("page, dim, tokens", [(1024, 16, 16), (2048, 32, 16), (2048, 16, 32), (4096, 16, 48)])
+def test_pages_smaller_than_the_controllers(cuda, bam, page, dim, tokens):
+    """Pages of 1 and 2 KiB: several slots, and several blocks of the store, in one page of the controller."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(29)
+    lens = [500, 0, 31, 90]
+    kv = make(bam, torch, sum(-(-n // tokens) for n in lens) + 5, 3, dim, torch.float16, page=page, slots=40, tokens=tokens, max_grid=4)
+    k, v, table = fill(torch, g, kv, lens)
+    order = torch.randperm(len(k), generator=g, device="cuda")
+    kv.append(k[order], v[order], order)
+    bk, bv = kv.gather(order)
+    assert torch.equal(bk, k[order]) and torch.equal(bv, v[order])
+    q = rand(torch, g, len(lens), 6, dim, dtype=torch.float16, scale=2.0)
+    out, lse = kv.attend(q, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), return_lse=True)
+    assert kv.cache.ctrl.status() == (0, "none", 0)
+    check_attend(torch, out, lse, attend64(torch, q, k, v, table, lens, tokens, dim ** -0.5), torch.float16)
+    done(kv)
