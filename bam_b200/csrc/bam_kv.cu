@@ -161,8 +161,9 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
  * Bytes bound it, every row is read and written once; what that needs is rows in flight: four rows of a lane are loaded before
  * the first is worked on (two: 164 us instead of 150).  It reaches 3.5 TB/s, 0.53 of a copy (111 us for 393 MB without the
  * gather): 16 warps an SM, all that 128 registers allow, wait for their loads in turn and issue in 40 % of the cycles;
- * a second row of keys in flight spilled (190 us), rows prefetched through shared memory, 96 KB a block, took 156 us instead
- * of 142. */
+ * a second row of keys in flight spilled far more than the 28 bytes a thread that the kernel spills as it is (190 us), rows
+ * prefetched through shared memory, 96 KB a block, took 156 us instead of 142.  200 tokens take 18 us in a graph, one token 13:
+ * the start and the end of a cooperative launch and the look-ups. */
 #define KV_ROWS_AHEAD 4
 
 /* VEC: every row, weight and angle lies on a 16-byte boundary. */
@@ -342,7 +343,8 @@ struct KvAppendWork {
  * Bytes bound it.  30001 tokens of 8 heads of 128 take 54 us, 4.6 TB/s: about 12 us of a launch that starts, looks its first
  * pages up and ends, and the rest at what a copy reaches.  Three blocks an SM, four rows of a lane loaded before the first
  * is stored (two: 65 us; eight at two blocks: 71).  Through shared memory with bulk copies, the look-ups of an item wait for
- * its one stage: 64 to 73 us. */
+ * its one stage: 64 to 73 us.  80 registers, for three blocks an SM, spill 52 bytes a thread.  An indexing kernel over plain
+ * tensors needs no look-up and takes 53 us; the rows of 200 tokens take 17 us in a graph. */
 template <bool VEC>
 struct KvGatherWork {
     static constexpr int threads = BAM_THREADS, min_blocks = 3;

@@ -25,17 +25,19 @@ namespace bam {
  * or more chunks under way for each (200 KB of an SM's shared memory).  The fourth warp of a block looks their pages
  * up and pins them up to 16 chunks ahead: a look-up is three dependent accesses that miss L2 while the rows stream
  * through it, 2 to 5 us (done by the workers themselves, 32 pages at a time, it cost 3 us of 186, and registers that
- * wide heads lack).  The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured):
+ * wide heads lack: 16 heads of 256 spill 32 to 44 bytes a thread as it is).  The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured):
  * up to 16 query heads are all there is, tcgen05 tiles of 64 or 128 rows would be mostly padding.  The scores have
  * the queries as rows and the sums as columns, S = Q K^T and O^T = V^T P^T: the scores are then where the second
  * product wants its right operand, and eight query heads take half of the instructions (and of the registers for O)
  * that sixteen do.  At 128 dimensions a chunk of 32 tokens takes 64 of them, 130 of the 710 cycles that HBM needs to
  * deliver it to an SM.
  *
- * Measured (bf16, 8 key/value heads of 128): 64 sequences of 2500 to 4100 tokens, 867 MB, 163 us = 5.3 TB/s, 0.81 of a copy
- * (6.7 TB/s between the first chunk and the last); 32 of 130 to 1700, 120 MB, 47 us.  What the short ones wait for: 3 us until
- * the list is laid out, 4 until the first pages are looked up and have landed, 9 chunks of 0.75 us a worker, 6 to 8 us from
- * a worker's last chunk to the end of its joins, 2 until the controller blocks have left.  A call costs the host 15 us. */
+ * Measured (bf16, 8 key/value heads of 128): 64 sequences of 2500 to 4100 tokens, 867 MB, 165 us = 5.2 TB/s, 0.80 of a copy;
+ * 32 of 130 to 1700, 120 MB, 47 us.  Time stamps of the latter's 744 workers, in us from the start of the first block: the list
+ * is laid out at 2.5; the first chunk has landed at 9.5 (mean; 16.6 the last); the last of 11 chunks is consumed at 26.1 (21.3
+ * to 34.3); the parts are written at 27.3 and joined at 33.9 (the last at 41.9); 5 more are the start of a cooperative launch
+ * and the end of the controller blocks.  In the large case the workers' last chunks lie between 112 and 152 us: equal runs do
+ * not end together.  A call costs the host 13 us. */
 #define KV_STAGES_MAX 8u              /* stages of a worker */
 #define KV_AHEAD 16u                  /* chunks of a worker that are pinned and not yet consumed, at most */
 #define KV_PIN_LANES 10u              /* lanes of the pinning warp for each worker */
