@@ -57,6 +57,7 @@ struct bam_ctrl {
 struct bam_cache {
     bam_ctrl* ctrl = nullptr;         /* the (first) backing controller: launches run with its descriptor */
     std::vector<bam_ctrl*> members;   /* all backing controllers when there are several */
+    int device = 0;                   /* kept apart from ctrl: handles may be destroyed in any order */
     bam_emu_qp_t* d_group_qps = nullptr;   /* controller-side state of all members' queues, contiguous */
     void* base_raw = nullptr;         /* the allocation d.base_addr (page-aligned) lies in */
     void* prp_lists_raw = nullptr;    /* the allocation d.prp_lists (page-aligned) lies in */
@@ -67,6 +68,7 @@ struct bam_cache {
 
 struct bam_array {
     bam_cache* pc = nullptr;
+    int device = 0;                     /* kept apart from pc: handles may be destroyed in any order */
     uint32_t elem_bytes = 0;
     uint64_t n_elems = 0;
     bam::range_d_t<uint64_t> h_range;   /* the first range; layout does not depend on the element type */

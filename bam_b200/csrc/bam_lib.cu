@@ -11,6 +11,7 @@
  */
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -814,6 +815,10 @@ extern "C" int bam_ctrl_create(bam_ctrl_t* out, int device, uint64_t store_bytes
 extern "C" int bam_ctrl_destroy(bam_ctrl_t c)
 {
     if (!c) return BAM_EINVAL;
+    if (c->group) {                                       /* the cache over it must not come back to it */
+        std::vector<bam_ctrl*>& m = c->group->members;
+        m.erase(std::remove(m.begin(), m.end(), c), m.end());
+    }
     cudaSetDevice(c->device);
     cudaDeviceSynchronize();
     cudaFree(c->arena);
@@ -1008,6 +1013,7 @@ extern "C" int bam_cache_create_multi(bam_cache_t* out, const bam_ctrl_t* ctrls,
     bam_cache* pc = new (std::nothrow) bam_cache();
     if (!pc) return BAM_ENOMEM;
     pc->ctrl = ctrl;
+    pc->device = ctrl->device;
     uint64_t want = (n_pages * 2 + 6) / 7;           /* load factor <= 0.5 over 7-entry buckets */
     pc->n_buckets = 1; while (pc->n_buckets < want) pc->n_buckets <<= 1;
     page_cache_d_t& d = pc->d;
@@ -1099,7 +1105,7 @@ extern "C" int bam_cache_create(bam_cache_t* out, bam_ctrl_t ctrl, uint32_t page
 extern "C" int bam_cache_destroy(bam_cache_t pc)
 {
     if (!pc) return BAM_EINVAL;
-    cudaSetDevice(pc->ctrl->device);
+    cudaSetDevice(pc->device);
     cudaDeviceSynchronize();
     cache_ungroup(pc);
     cache_free_device(pc);
@@ -1205,7 +1211,7 @@ extern "C" int bam_array_create_ranges(bam_array_t* out, bam_cache_t pc, uint64_
     CK(cudaSetDevice(pc->ctrl->device));
     bam_array* a = new (std::nothrow) bam_array();
     if (!a) return BAM_ENOMEM;
-    a->pc = pc; a->elem_bytes = elem_bytes; a->n_elems = n_elems; a->n_ranges = n_ranges;
+    a->pc = pc; a->device = pc->device; a->elem_bytes = elem_bytes; a->n_elems = n_elems; a->n_ranges = n_ranges;
     a->h_range = h[0];
     struct { uint64_t n_elems, start_offset, n_ranges; void* d_ranges; } h_arr;
     cudaError_t e = cudaMalloc(&a->d_range, sizeof(range_d_t<uint64_t>) * n_ranges);
@@ -1239,7 +1245,7 @@ extern "C" int bam_array_create(bam_array_t* out, bam_cache_t pc, uint64_t n_ele
 extern "C" int bam_array_destroy(bam_array_t a)
 {
     if (!a) return BAM_EINVAL;
-    cudaSetDevice(a->pc->ctrl->device);
+    cudaSetDevice(a->device);
     cudaDeviceSynchronize();
     cudaFree(a->d_range); cudaFree(a->d_array);
     delete a;

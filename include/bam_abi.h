@@ -106,7 +106,8 @@ int bam_cache_create(bam_cache_t* out, bam_ctrl_t ctrl, uint32_t page_size, uint
  * queues of all of them, they report into the first controller's status block (bam_ctrl_status of
  * any member reads it) and bam_ctrl_configure of the FIRST controller sets the launch geometry.
  * A controller can back one multi-controller cache at a time (BAM_EBUSY otherwise); destroy the
- * cache before its controllers.  How a range's pages map to the controllers is chosen per array:
+ * cache before its controllers (once one of them is gone, destroying is all that the cache and its
+ * arrays may be used for).  How a range's pages map to the controllers is chosen per array:
  * bam_array_create_dist. */
 int bam_cache_create_multi(bam_cache_t* out, const bam_ctrl_t* ctrls, uint32_t n_ctrls, uint32_t page_size,
                            uint64_t n_pages);
