@@ -29,6 +29,8 @@ class KvCache:
     multiple of 16).  A token's slot is block * block_tokens + its place in the block.  `dist` lays the pages over the
     controllers of the cache (REPLICATE or STRIPE), store_byte_offset places them in the store.
 
+    While Controller.status() says that something went wrong, calls do nothing and their results are undefined.
+
     The calls run on the current stream of the cache's device or on `stream` (a torch stream or a raw handle), in whose
     memory pool their results are; the order between streams, and that tensors live long enough, is the caller's affair as
     for any work on another stream.  (The per-thread default stream is refused: its handle is the same number in every
@@ -116,6 +118,14 @@ class KvCache:
         if (n > 1 and stride[0] < self.head_dim) or (heads > 1 and stride[1] < self.head_dim):
             raise ValueError(f"the rows of {name} lie on one another")
         return stride
+
+    @staticmethod
+    def _changed(*tensors):
+        """The caller's tensors that a launch writes: autograd is to notice if it has saved them."""
+        import torch
+        for t in tensors:
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
 
     def _flat(self, name, t, dtype, n):
         """The address of n contiguous values."""
@@ -213,7 +223,7 @@ class KvCache:
         q_w = None if q_norm is None else self._flat("q_norm", q_norm, self.dtype, self.head_dim)
         k_w = None if k_norm is None else self._flat("k_norm", k_norm, self.dtype, self.head_dim)
         layout = self._layout(layer)
-        q_at = out_at = None
+        q_at = out_at = given = None
         heads, q_stride, out_stride = 0, _NO_STRIDE, _NO_STRIDE
         if q is None:
             if q_norm is not None or q_out is not None:
@@ -228,11 +238,14 @@ class KvCache:
                 out_stride = heads * self.head_dim, self.head_dim
             else:
                 out_stride = self._rows("q_out", q_out, n, heads)
+                given = q_out
             q_at, out_at = q.data_ptr(), q_out.data_ptr()
         if n:
             a = KvAppend(q_at, k.data_ptr(), v.data_ptr(), out_at, q_stride, k_stride, v_stride, out_stride, n, at, *turn[:5],
                          q_w, k_w, heads, turn[5], turn[6], norm_eps)
             self._call(self.lib.bam_launch_kv_append, layout, C.byref(a))
+            if given is not None:
+                self._changed(given)
         return q_out
 
     def gather(self, slots, layer=0, out=None, stream=None):
@@ -254,6 +267,8 @@ class KvCache:
             vs = (C.c_int64 * 2)(*self._rows("out[1]", v, n, self.n_kv_heads))
         if n:
             self._call(self.lib.bam_launch_kv_gather, layout, n, at, k.data_ptr(), v.data_ptr(), ks, vs)
+            if out is not None:
+                self._changed(k, v)
         return k, v
 
     def attend(self, q, block_table, seq_lens, layer=0, scale=None, window=0, sinks=0, out=None, return_lse=False, stream=None):
@@ -282,6 +297,7 @@ class KvCache:
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
         layout = self._layout(layer)
+        given = out
         if out is None:
             out = torch.empty((n, heads, self.head_dim), dtype=self.dtype, device=self.device)
             out_stride = heads * self.head_dim, self.head_dim
@@ -293,4 +309,6 @@ class KvCache:
                          lens, stride[0], min(window, 1 << 62), min(sinks, 1 << 62), n, heads, width,
                          self.head_dim ** -0.5 if scale is None else scale)
             self._call(self.lib.bam_launch_kv_attend, layout, C.byref(a))
+            if given is not None:
+                self._changed(given)
         return (out, lse) if return_lse else out
