@@ -338,3 +338,50 @@ def test_pages_smaller_than_the_controllers(cuda, bam, page, dim, tokens):
     assert kv.cache.ctrl.status() == (0, "none", 0)
     check_attend(torch, out, lse, attend64(torch, q, k, v, table, lens, tokens, dim ** -0.5), torch.float16)
     done(kv)
+
+
+def test_a_bad_index_leaves_the_other_rows_right(cuda, bam):
+    """What an index outside its range concerns is undefined, and nothing else: other tokens, sequences and pages."""
+    torch = cuda
+    g = torch.Generator(device="cuda").manual_seed(30)
+    lens = [300, 77, 150, 40]
+    kv = make(bam, torch, sum(-(-n // 16) for n in lens) + 4, 2, 64, torch.bfloat16, page=4096)
+    k, v, table = fill(torch, g, kv, lens)
+    total = len(k)
+    kv.append(k, v, torch.arange(total, device="cuda"))
+    q = rand(torch, g, 4, 8, 64, dtype=torch.bfloat16, scale=2.0)
+    ls = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse, tol, ltol = attend64(torch, q, k, v, table, lens, 16, 0.125)
+    for what in ("block", "length"):
+        bad_t, bad_l = table.clone(), ls.clone()
+        if what == "block":
+            bad_t[1, 2] = kv.n_blocks
+        else:
+            bad_l[1] = 1 << 30
+        o, s = kv.attend(q, bad_t, bad_l, return_lse=True)
+        assert kv.cache.ctrl.status(clear=True)[:2] == (34, "range")
+        rest = torch.tensor([0, 2, 3], device="cuda")
+        check_attend(torch, o[rest], s[rest], (out[rest], lse[rest], tol[rest], ltol[rest]), torch.bfloat16)
+    # append: token 5 has no such slot, token 9 no such position
+    n = 40
+    nk, nv, nq = (rand(torch, g, n, h, 64, dtype=torch.bfloat16) for h in (2, 2, 4))
+    slots = torch.randperm(total, generator=g, device="cuda")[:n]
+    was, pos = slots.clone(), torch.arange(n, device="cuda")
+    cos, sin = torch.ones(n, 32, device="cuda"), torch.zeros(n, 32, device="cuda")
+    slots[5], pos[9] = total, n
+    got = kv.append(nk, nv, slots, positions=pos, rope=(cos, sin), q=nq)
+    assert kv.cache.ctrl.status(clear=True)[:2] == (34, "range")
+    good = torch.tensor([i for i in range(n) if i not in (5, 9)], device="cuda")
+    assert torch.equal(got[good], nq[good])
+    k[was[good]], v[was[good]] = nk[good], nv[good]
+    every = torch.arange(total, device="cuda")
+    kept = every != was[9]                                       # the row whose position is none
+    bk, bv = kv.gather(every)
+    assert torch.equal(bk[kept], k[kept]) and torch.equal(bv[kept], v[kept])
+    every[3] = -total
+    every[7] = total + 5
+    bk, bv = kv.gather(every)
+    assert kv.cache.ctrl.status(clear=True)[:2] == (34, "range")
+    kept[7] = kept[3] = False
+    assert torch.equal(bk[kept], k[kept]) and torch.equal(bv[kept], v[kept]) and not bk[3].any() and not bv[3].any()
+    done(kv)
