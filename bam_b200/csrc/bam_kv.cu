@@ -153,7 +153,8 @@ BAM_DEV bool kv_with_pages(const kv_layout_d_t& L, bool want, uint64_t page, boo
  * consecutive tokens, then q_heads of the query heads of q_tokens tokens.  A run is the tokens in a row that go to one
  * block: one warp writes its share of it, to the end of the run and not of the item, and pins each page once.  (Warps that
  * miss the same page at once claim a slot each: a prompt whose pages were written by two warps each evicted half of a cache
- * with room for all.)  Items differ in length, hence the drawing; which warp writes a row changes nothing in it.
+ * with room for all.  The price is paid by large blocks, resident or not: with 1024 tokens a block, 16000 tokens of 8 heads
+ * are work for 128 warps.)  Items differ in length, hence the drawing; which warp writes a row changes nothing in it.
  * Items are as large as still makes enough of them: a warp pins its pages together and loads angles and weights once an
  * item.  16000 tokens of 32 + 8 heads of 128, gathered again: 144 us with items of 32 and 4 heads, 152 with 16 and 1, 170 with
  * 8 query heads (which are too few rows in flight); 777 tokens of 15 + 3 heads of 256: 33 us with 1 key/value head, 37 with

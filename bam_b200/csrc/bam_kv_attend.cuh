@@ -25,9 +25,9 @@ namespace bam {
  * or more chunks under way for each (200 KB of an SM's shared memory).  The fourth warp of a block looks their pages
  * up and pins them up to 16 chunks ahead: a look-up is three dependent accesses that miss L2 while the rows stream
  * through it, 2 to 5 us (done by the workers themselves, 32 pages at a time, it cost 3 us of 186, and registers that
- * wide heads lack: 16 heads of 256 spill 32 to 44 bytes a thread as it is).  The products go through m16n8k16 matrix instructions (8.3 cycles each per quarter SM, measured):
- * up to 16 query heads are all there is, tcgen05 tiles of 64 or 128 rows would be mostly padding.  The scores have
- * the queries as rows and the sums as columns, S = Q K^T and O^T = V^T P^T: the scores are then where the second
+ * wide heads lack: 16 heads of 256 spill 32 to 44 bytes a thread as it is).  The products go through m16n8k16 matrix
+ * instructions (8.3 cycles each per quarter SM, measured): up to 16 query heads are all there is, tcgen05 tiles of 64 or 128
+ * rows would be mostly padding.  The scores have the queries as rows and the sums as columns, S = Q K^T and O^T = V^T P^T: the scores are then where the second
  * product wants its right operand, and eight query heads take half of the instructions (and of the registers for O)
  * that sixteen do.  At 128 dimensions a chunk of 32 tokens takes 64 of them, 130 of the 710 cycles that HBM needs to
  * deliver it to an SM.
@@ -439,9 +439,9 @@ struct KvAttendWork {
 
     /* One chunk: S = Q K^T, p = 2^((S - m) scale log2(e)), O^T += V^T p^T.  m is a maximum of S as it is, and the difference
      * comes before the scale: the largest weight is 1 however large the scores are.  (With a scaled m it would be 2 to the
-     * rounding of m, anything beyond 2^24.)  The weights go into the product as two 16-bit
-     * parts, kv_type::weight p = hi + lo, which keeps 16 bits of them (bf16), or 21 and what is above 2^-40 (fp16): the
-     * product runs twice, on a pipe that idles.  The sums are of the same scale, the denominator counts p itself.
+     * rounding of m, anything beyond 2^24.)  The weights go into the product as two 16-bit parts,
+     * kv_type::weight p = hi + lo, which keeps 16 bits of them (bf16), or 21 and what is above 2^-40 (fp16): the product
+     * runs twice, on a pipe that idles.  The sums are of the same scale, the denominator counts p itself.
      * An infinite value makes its sum infinite, if its weight is any number but 0 in 32 bits: infinity x 0, of a part that
      * is 0, and infinities of different sign, of parts of different sign, would make it NaN.  So hi is never 0 (lo takes what
      * is too much back) and lo is multiplied with values cut to the finite range.

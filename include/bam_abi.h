@@ -367,9 +367,8 @@ int bam_ctrl_write_store_from_device(bam_ctrl_t c, uint64_t byte_offset, const v
  * thread's device as it was.  scratch_dev: bam_kv_scratch_bytes bytes of device memory, 128-byte aligned, set up once
  * by bam_kv_scratch_init.  Every launch leaves it ready for the next, also one that fails; launches that may run at the
  * same time need one each: one for every stream (the handle cudaStreamPerThread is another stream in every thread), one for
- * every captured graph.  An index outside its range (a slot,
- * position, block or length) is not followed: the status block says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has
- * finished, the rows that it concerns are undefined.  While the status block says anything, launches do nothing. */
+ * every captured graph.  An index outside its range (a slot, position, block or length) is not followed: the status block
+ * says BAM_ERANGE (where: BAM_AT_RANGE) when the launch has finished, the rows that it concerns are undefined.  While the status block says anything, launches do nothing. */
 #define BAM_KV_BF16 0u
 #define BAM_KV_FP16 1u
 #define BAM_KV_ROPE_HALF 0u      /* pairs (i, i + rotary_dim / 2) */
@@ -418,8 +417,8 @@ int bam_launch_kv_gather(bam_array_t a, const bam_kv_layout_t* layout, uint64_t 
  * first `sinks`.  Query head h reads key/value head h / (n_q_heads / n_kv_heads).  Token j of sequence b lies in block
  * block_table[b * table_stride + j / block_tokens] (int32); entries of blocks without a visible token are not read.
  * Nothing visible: zeros, and an lse of -infinity (lse: batch x n_q_heads floats, or NULL).  An infinite value of a visible
- * token makes its element of out infinite (NaN with one of the other sign, or if p_j is below 2^-126).  out may be q.  A cache
- * of a single slot is refused where block_tokens is no multiple of 32: two blocks are read together there. */
+ * token makes its element of out infinite (NaN with one of the other sign, or if p_j is below 2^-126).  out may be q.  32 tokens
+ * are read together for most head_dims: a cache of a single slot is refused where they lie in two blocks. */
 typedef struct {
     const void* q;
     void* out;
